@@ -24,6 +24,9 @@
  *                   (uint8 codes, fp32 nested scales, fp32 offsets, 256-entry
  *                   code table), decoded inside the GEMMs
  *   NF4_DQ_KN       NF4_DQ for a weight stored [E, in, out] (as NF4_F32_KN)
+ *   MXFP4 weight    codes [E, out, in/2] uint8 (e2m1, element 2 i of a row in the
+ *                   low nibble of byte i), `scale` uint8 [E, out, in/32]: the
+ *                   biased exponent of the power of two of 32 elements (255: NaN)
  *   NF4_F32_KN      the same codes and fp32 absmax for a weight stored
  *                   [E, in, out] (y = x @ W[e], the MAGI-2 group layout of
  *                   magi2_preview.py:2680-2704): codes [E, in, out/2] packed
@@ -69,6 +72,7 @@ extern "C" {
 #define MX_FMT_NF4_F32_KN 5  /* NF4_F32 stored [E, in, out], blocks along out (MAGI-2 groups) */
 #define MX_FMT_NF4_DQ 6      /* NF4 codes with the two-level absmax of a bitsandbytes payload */
 #define MX_FMT_NF4_DQ_KN 7   /* NF4_DQ stored [E, in, out], blocks along out */
+#define MX_FMT_MXFP4 8       /* OCP microscaled e2m1, one power of two per 32 columns */
 
 /*
  * Two-level (double-quantised) absmax of an MX_FMT_NF4_DQ / _DQ_KN weight, as a
@@ -413,6 +417,26 @@ int mx_int8_quantize(const void *w, int w_dtype, int64_t rows, int64_t cols, int
 int mx_int8_dequantize(const int8_t *q, const void *scale, int64_t rows, int64_t cols,
                        void *out, int out_dtype, void *stream);
 
+/*
+ * MXFP4 (OCP Microscaling Formats 1.0: e2m1 elements, e8m0 scales, blocks of 32
+ * along a row). Rows of `cols` elements (any number >= 1), `ldx` elements apart,
+ * bf16 or fp32. B = ceil(cols / 32) blocks per row:
+ *   X = 2^clamp(floor(log2 max|x|) - 2, -127, 125)
+ *   element = x / X rounded to nearest (ties to even) on 0, .5, 1, 1.5, 2, 3, 4, 6
+ *             and their negatives, above 6 to 6
+ * codes [rows, 16 B] uint8 (element 2 i in the low nibble of byte i; elements past
+ * cols are zero), scales [rows, B] uint8 (log2 X + 127). A block that holds a NaN or
+ * an infinity gets scale 255 and zero codes, and reads back as NaN. codes 4-byte
+ * aligned.
+ */
+int mx_mxfp4_quantize(const void *x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx,
+                      uint8_t *codes, uint8_t *scales, void *stream);
+
+/* out [rows, cols] (bf16 or fp32) = element * X: exact in fp32 unless it overflows
+ * (scales above 252), and in bf16 likewise. codes 4-byte aligned. */
+int mx_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols,
+                        void *out, int out_dtype, void *stream);
+
 /* ------------------------------------------------------------------------ */
 /* Grouped expert GEMMs and the fused layer                                   */
 /* ------------------------------------------------------------------------ */
@@ -707,6 +731,27 @@ int mx_grouped_linear(const void *x, const int64_t *counts, int64_t num_rows, in
                       const mx_weight *w, const mx_lora *lora, void *out, void *workspace,
                       void *stream);
 
+/* Bytes of scratch for mx_mxfp4_grouped_linear (0: invalid sizes). */
+size_t mx_mxfp4_grouped_linear_workspace_size(int64_t num_rows, int num_experts,
+                                              int64_t in_features);
+
+/*
+ * One grouped projection with both operands in MXFP4: the rows x [S, in] (bf16 or
+ * fp32) are quantised as mx_mxfp4_quantize does and multiplied with an MX_FMT_MXFP4
+ * weight on the scaled matrix instructions,
+ *   out[i][n] = sum over blocks b of 2^(sx[i][b] + sw[n][b] - 254)
+ *               * sum over the block's elements of cx * cw,
+ * accumulated in fp32, for the expert owning row i: `offsets` [E] holds each
+ * expert's inclusive row end, int32 or int64 (offsets_64). out [S, out] bf16 or
+ * fp32. Ends that decrease or pass num_rows are clamped, and counted into the int32
+ * at the head of the workspace, as are rows past the last end, which are left as
+ * they were; host_err (mapped pinned memory or NULL) receives the count too.
+ * in_features a multiple of 64, out_features of 8.
+ */
+int mx_mxfp4_grouped_linear(const void *x, int x_dtype, const void *offsets, int offsets_64,
+                            int64_t num_rows, int num_experts, const mx_weight *w, void *out,
+                            int out_dtype, void *workspace, int32_t *host_err, void *stream);
+
 /* Bytes of scratch for mx_grouped_linear_backward. */
 size_t mx_grouped_linear_backward_workspace_size(int64_t num_rows, int num_experts,
                                                  int64_t in_features, int64_t out_features,
@@ -724,7 +769,7 @@ size_t mx_grouped_linear_backward_workspace_size(int64_t num_rows, int num_exper
  * dX = grouped_mm(dY, W) over the re-dequantised weight) plus the autograd of
  * ActiveExpertLoRA.grouped_forward (active_expert_lora.py:348-399), the
  * backward of CompressedGroupedExperts.grouped_linear (experts.py:803-827).
- * in_features and out_features are multiples of 64; BF16, NF4, NF4_F32 and
+ * in_features and out_features are multiples of 64; BF16, NF4, NF4_F32, MXFP4 and
  * INT8 weights.
  */
 int mx_grouped_linear_backward(const void *grad_out, const void *x, const int64_t *counts,
@@ -773,6 +818,63 @@ int mx_moe_backward_act(const void *grad_out, int grad_dtype, const void *tokens
 /* Bytes of scratch for mx_moe_backward (and mx_moe_backward_act). */
 size_t mx_moe_backward_workspace_size(int64_t num_tokens, int top_k, int num_experts,
                                       int64_t hidden, int64_t ffn, int lora_rank);
+
+/* ------------------------------------------------------------------------ */
+/* Adapter training: the optimiser step                                      */
+/* ------------------------------------------------------------------------ */
+
+/* One tensor of an AdamW step: n elements of p (updated) and g at device
+ * addresses, its moments from position `at` on of the flat moments (a multiple of
+ * 128; the positions up to the next multiple of 128 past its end are its padding),
+ * `index` its entry of the device steps and scalars (capturable steps). */
+typedef struct mx_adamw_tensor {
+  void *p;
+  const void *g;
+  int64_t n;
+  int64_t at;
+  int64_t index;
+} mx_adamw_tensor;
+
+typedef struct mx_adamw_config {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;            /* the step being taken, from 1 on (unused when capturable) */
+  uint32_t seed;           /* 8-bit moments: seed and group of the rounding noise */
+  uint32_t group;
+  int dtype;               /* of p and g: MX_DTYPE_* */
+  int state_bits;          /* 32 or 8 */
+  void *exp_avg;           /* flat moments: fp32 [total], or uint8 codes [total] */
+  void *exp_avg_sq;
+  uint8_t *exp_avg_e;      /* 8-bit moments: block exponents [total / 128] */
+  uint8_t *exp_avg_sq_e;
+  int64_t *steps;          /* capturable: device steps taken, one per tensor, else NULL */
+  void *scalars;           /* capturable: 32 bytes of device scratch per tensor */
+  const float *lr_ptr;     /* capturable: device learning rate, or NULL for lr */
+} mx_adamw_config;
+
+/*
+ * AdamW over `count` tensors in a few launches. Per element, in fp32:
+ *   m' = b1 m + (1 - b1) g,  v' = b2 v + ((1 - b2) g) g   (each operation rounded)
+ *   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+ * p' rounded to p's dtype. 8-bit moments are blocks of 128 elements with one
+ * exponent E = clamp(floor(log2 max|.|), -126, 126) (stored + 127; 255 where the
+ * block holds a NaN or an infinity, which reads back as NaN throughout): m is a
+ * sign, 4 exponent and 3 fraction bits, v 5 exponent and 3 fraction bits, both
+ * with every code finite and 1.875 * 2^E the largest. They are rounded
+ * stochastically: of mix(position + key) the low 16 bits decide m's rounding and the
+ * high 16 bits v's, where key = mix(mix(seed) + t), mixed once more, as mix(key + w),
+ * with a group w that is not 0 and then with an upper half w of the position that is
+ * not 0, and mix(x) is x = (x ^ x >> 16) * 0x9E3779B9; x = (x ^ x >> 15) * 0xBB67AE85;
+ * x ^ x >> 16 in 32 bits. p' is formed from the moments before they are rounded.
+ * With `steps` the step counts live on the device and are advanced by the call, so
+ * that it can be captured into a graph and replayed.
+ */
+int mx_adamw_step(const mx_adamw_tensor *tensors, int count, const mx_adamw_config *config,
+                  void *stream);
+
+/* fp32 values [n] of 8-bit moments from position 0 on (n a multiple of 128);
+ * is_signed: codes of m, else of v. */
+int mx_adamw_moments(const uint8_t *codes, const uint8_t *exponents, int64_t n, int is_signed,
+                     float *out, void *stream);
 
 #ifdef __cplusplus
 }

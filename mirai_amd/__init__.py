@@ -25,6 +25,8 @@ from .magi2 import (
     read_reference_magi2_artifact,
     route_topk_heads,
 )
+from .mxfp4 import MXFP4Tensor, mxfp4_dequantize, mxfp4_quantize
+from .optim import AdapterAdamW
 from .router import FusedRouter, fused_router_forward, router_weight_planes
 from .routing import route_topk
 from .specs import (
@@ -36,6 +38,7 @@ from .specs import (
 
 __all__ = [
     "ActiveExpertLoRA",
+    "AdapterAdamW",
     "CANONICAL_PACKED_EXPERT_MLP_SPEC",
     "CompressedGroupedExperts",
     "DispatchPlan",
@@ -43,6 +46,7 @@ __all__ = [
     "RouteIndexError",
     "ExpertMLPExecutionSpec",
     "ExpertProjectionRole",
+    "MXFP4Tensor",
     "Magi2FusedMoEBackend",
     "Magi2GroupedExperts",
     "Magi2QuantizedExpertError",
@@ -57,6 +61,8 @@ __all__ = [
     "fused_router_forward",
     "load_reference_magi2_artifact",
     "lora_scale",
+    "mxfp4_dequantize",
+    "mxfp4_quantize",
     "permute_routed_tokens",
     "read_reference_magi2_artifact",
     "route_topk",

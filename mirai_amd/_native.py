@@ -7,11 +7,13 @@ raises :class:`NativeLibraryError` when the library or a GPU is missing.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
 import time
-from ctypes import POINTER, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import (POINTER, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32,
+                    c_void_p)
 from pathlib import Path
 from typing import Any
 
@@ -34,6 +36,7 @@ FMT_NF4_F32 = 4    # NF4 codes with an fp32 block absmax (ingested bitsandbytes 
 FMT_NF4_F32_KN = 5  # the same, stored [E, in, out] with the blocks along out (MAGI-2 groups)
 FMT_NF4_DQ = 6     # NF4 codes with a bitsandbytes two-level absmax decoded in the GEMMs
 FMT_NF4_DQ_KN = 7  # the same, stored [E, in, out]
+FMT_MXFP4 = 8      # microscaled e2m1 codes, one power of two per 32 columns
 
 LAUNCH_128 = 0     # mx_gemm_launch: how a grouped GEMM is tiled
 LAUNCH_STREAM = 1
@@ -94,6 +97,21 @@ class MxNf4Dq(ctypes.Structure):
 
 class MxLora(ctypes.Structure):
     _fields_ = [("a", c_void_p), ("b", c_void_p), ("rank", c_int), ("scale", c_float)]
+
+
+class MxAdamwTensor(ctypes.Structure):
+    _fields_ = [("p", c_void_p), ("g", c_void_p), ("n", c_int64), ("at", c_int64),
+                ("index", c_int64)]
+
+
+class MxAdamwConfig(ctypes.Structure):
+    _fields_ = [
+        ("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double),
+        ("weight_decay", c_double), ("step", c_int64), ("seed", c_uint32), ("group", c_uint32),
+        ("dtype", c_int), ("state_bits", c_int), ("exp_avg", c_void_p), ("exp_avg_sq", c_void_p),
+        ("exp_avg_e", c_void_p), ("exp_avg_sq_e", c_void_p), ("steps", c_void_p),
+        ("scalars", c_void_p), ("lr_ptr", c_void_p),
+    ]
 
 
 _P = c_void_p
@@ -160,6 +178,13 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "mx_nf4_dq_absmax": (c_int, [POINTER(MxNf4Dq), c_int64, c_int64, _P, _P]),
     "mx_int8_quantize": (c_int, [_P, c_int, c_int64, c_int64, _P, _P, _P]),
     "mx_int8_dequantize": (c_int, [_P, _P, c_int64, c_int64, _P, c_int, _P]),
+    "mx_mxfp4_quantize": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, _P, _P]),
+    "mx_mxfp4_dequantize": (c_int, [_P, _P, c_int64, c_int64, _P, c_int, _P]),
+    "mx_mxfp4_grouped_linear_workspace_size": (c_size_t, [c_int64, c_int, c_int64]),
+    "mx_mxfp4_grouped_linear": (
+        c_int, [_P, c_int, _P, c_int, c_int64, c_int, _W, _P, c_int, _P, _P, _P]),
+    "mx_adamw_step": (c_int, [_P, c_int, POINTER(MxAdamwConfig), _P]),
+    "mx_adamw_moments": (c_int, [_P, _P, c_int64, c_int, _P, _P]),
     "mx_set_stage_events": (c_int, [POINTER(c_void_p), c_int]),
     "mx_moe_workspace_size": (c_size_t, [c_int64, c_int, c_int, c_int64, c_int64, c_int]),
     "mx_gemm_launch": (c_int, [c_int, c_int, c_int64, c_int64, c_int]),
@@ -280,6 +305,13 @@ def stream(device: torch.device) -> int:
     index = device.index
     return torch._C._cuda_getCurrentRawStream(
         torch.cuda.current_device() if index is None else index)
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one, for launches on its streams."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

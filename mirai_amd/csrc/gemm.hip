@@ -47,8 +47,14 @@ constexpr bool is_dq(int fmt) { return fmt == MX_FMT_NF4_DQ || fmt == MX_FMT_NF4
 constexpr bool is_nf4(int fmt) {
   return fmt == MX_FMT_NF4 || fmt == MX_FMT_NF4_F32 || fmt == MX_FMT_NF4_F32_KN || is_dq(fmt);
 }
+// OCP microscaled 4-bit floats: e2m1 codes, element 2 i of a row in the low nibble
+// of byte i, and one power of two (its biased exponent, a byte) per 32 columns.
+constexpr bool is_mx4(int fmt) { return fmt == MX_FMT_MXFP4; }
+// Formats of two codes per byte.
+constexpr bool is_code4(int fmt) { return is_nf4(fmt) || is_mx4(fmt); }
 constexpr bool f32_absmax(int fmt) { return fmt == MX_FMT_NF4_F32 || fmt == MX_FMT_NF4_F32_KN; }
-// Bytes of one block's absmax entry (DQ: the uint8 code).
+// Bytes of one block's absmax entry (DQ: the uint8 code; MXFP4: the two scales of
+// 64 columns).
 constexpr int absmax_bytes(int fmt) { return f32_absmax(fmt) ? 4 : is_dq(fmt) ? 1 : 2; }
 // Weights stored [E, in, out] with the NF4 blocks along out (a MAGI-2 packed
 // group, x @ W[g]): the forward reads them as the backward reads [E, out, in]
@@ -330,6 +336,24 @@ __device__ __forceinline__ void nf4_decode8(const Nf4Table &t, uint32_t c, uint3
   out[3] = __builtin_amdgcn_perm(ho, lo_, 0x07030602u);  // e6, e7
 }
 
+// The scale of one MXFP4 block as fp32: byte `i` of `raw`. 2^-127 (byte 0) is an
+// fp32 denormal; byte 255 gives a NaN.
+__device__ __forceinline__ float mx4_scale(uint32_t raw, int i) {
+  const uint32_t e = (raw >> (8 * i)) & 0xffu;
+  return __uint_as_float(e == 0 ? 0x00400000u : e == 255 ? 0x7fc00000u : e << 23);
+}
+
+// Eight e2m1 codes (one packed dword, element 0 in the low nibble) times their
+// block's scale -> four dwords of bf16 pairs in element order, exactly: two
+// elements per v_cvt_scalef32_pk_bf16_fp4, against 16 instructions of table
+// lookup per eight NF4 codes.
+__device__ __forceinline__ void mx4_decode8(uint32_t c, float scale, uint32_t *out) {
+  out[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0));
+  out[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1));
+  out[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2));
+  out[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3));
+}
+
 // LoRA factor tiles of the epilogue (one [BN][32] tile per adapter).
 template <int EPI, bool LORA, class T>
 constexpr int lora_tile_bytes() {
@@ -504,7 +528,7 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
   float b_scale = 0.0f;
   if (b_valid) {
     const uint8_t *w = static_cast<const uint8_t *>(pick(p.w, which));
-    if (is_nf4(FMT)) {
+    if (is_code4(FMT)) {
       b_base = w + wrow * (row_k / 2) + bh * (T::B_ELEMS / 2);
       b_absmax = static_cast<const uint8_t *>(pick(p.wscale, which)) +
                  wrow * (row_k / kNf4Block) * absmax_bytes(FMT);
@@ -545,10 +569,11 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
   }
 
   // Bytes of B per thread per stage, in 16-byte registers.
-  constexpr int kBBytes = is_nf4(FMT) ? T::B_ELEMS / 2
+  constexpr int kBBytes = is_code4(FMT) ? T::B_ELEMS / 2
                                             : (FMT == MX_FMT_INT8 ? T::B_ELEMS : T::B_ELEMS * 2);
   constexpr int kBRegs = kBBytes / 16;
-  constexpr int kBStageBytes = is_nf4(FMT) ? BK / 2 : (FMT == MX_FMT_INT8 ? BK : BK * 2);
+  static_assert(!is_mx4(FMT) || BK == 64, "an MXFP4 scale entry covers one stage");
+  constexpr int kBStageBytes = is_code4(FMT) ? BK / 2 : (FMT == MX_FMT_INT8 ? BK : BK * 2);
   // B packed data: two register sets (stage kt+1 is decoded while kt+2 loads).
   struct BRegs {
     u32x4 q[kBRegs];
@@ -577,7 +602,11 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
       const uint8_t *w = static_cast<const uint8_t *>(second ? p.w[1] : p.w[0]);
       const void *ws = second ? p.wscale[1] : p.wscale[0];
       const int64_t wrow = static_cast<int64_t>(e) * (second ? p.wn[1] : p.wn[0]) + krow;
-      if (is_nf4(FMT)) {
+      if (is_mx4(FMT)) {
+        // The lane's 32 columns are one block.
+        rb.q[0] = *reinterpret_cast<const u32x4 *>(w + wrow * (p.N / 2) + t_col0 / 2);
+        rb.abs = static_cast<const uint8_t *>(ws)[wrow * (p.N / 32) + t_col0 / 32];
+      } else if (is_nf4(FMT)) {
         rb.q[0] = *reinterpret_cast<const u32x4 *>(w + wrow * (p.N / 2) + t_col0 / 2);
         rb.abs = load_absmax<FMT>(ws, wrow * (p.N / kNf4Block) + t_col0 / kNf4Block);
         if (is_dq(FMT)) {
@@ -609,7 +638,7 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
 #pragma unroll
       for (int q = 0; q < kBRegs; ++q)
         rb.q[q] = *reinterpret_cast<const u32x4 *>(bb + static_cast<int64_t>(ks) * kBStageBytes + 16 * q);
-      rb.abs = is_nf4(FMT) ? load_absmax<FMT>(ba, ks * BK / kNf4Block) : 0u;
+      rb.abs = is_code4(FMT) ? load_absmax<FMT>(ba, ks * BK / kNf4Block) : 0u;
     } else {
 #pragma unroll
       for (int q = 0; q < kBRegs; ++q) rb.q[q] = u32x4{0u, 0u, 0u, 0u};
@@ -657,11 +686,14 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
       const int c = part * kChunksPerPart + cc;  // output chunk: 8 elements
       uint32_t d[4];
       const float sc = TRANS ? bf16_bits_to_f32(rb.abs) : b_scale;
-      if (is_nf4(FMT)) {
+      if (is_code4(FMT)) {
         // chunk c = code bytes 4c..4c+3 = dword c of the packed registers
         const u32x4 v = rb.q[c >> 2];
         const uint32_t word = (c & 3) == 0 ? v[0] : (c & 3) == 1 ? v[1] : (c & 3) == 2 ? v[2] : v[3];
-        nf4_decode8(t, word, d);
+        if constexpr (is_mx4(FMT))
+          mx4_decode8(word, mx4_scale(rb.abs, TRANS ? 0 : (chunk0 + c) >> 2), d);
+        else
+          nf4_decode8(t, word, d);
       } else if (FMT == MX_FMT_INT8) {
         // chunk c = int8 bytes 8c..8c+7 = dwords 2c, 2c+1
         const u32x4 v = rb.q[c >> 1];
@@ -1310,7 +1342,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr bool stream_format(int fmt) {
   return fmt == MX_FMT_NF4 || fmt == MX_FMT_NF4_F32 || fmt == MX_FMT_NF4_DQ ||
-         fmt == MX_FMT_INT8 || fmt == MX_FMT_BF16;
+         fmt == MX_FMT_INT8 || fmt == MX_FMT_BF16 || fmt == MX_FMT_MXFP4;
 }
 template <int FMT, int EPI>
 constexpr bool stream_capable() {
@@ -1395,7 +1427,7 @@ __device__ __forceinline__ void stream_tile(const Params &p, int2 tile, int nt, 
   const int64_t wrow = static_cast<int64_t>(e) * pick(p.wn, which) + n_row;
   // Bytes of one lane's share of a step, its 16-byte registers and the row's
   // bytes per step.
-  constexpr int kLaneBytes = is_nf4(FMT) ? KS / 4 : FMT == MX_FMT_INT8 ? KS / 2 : KS;
+  constexpr int kLaneBytes = is_code4(FMT) ? KS / 4 : FMT == MX_FMT_INT8 ? KS / 2 : KS;
   constexpr int kQ = kLaneBytes / 16;
   // bf16: a lane's 16-byte pieces lie 32 bytes apart (MFMA step s, half h at
   // 32 s + 16 h); the others take kLaneBytes in a row and exchange halves.
@@ -1405,7 +1437,7 @@ __device__ __forceinline__ void stream_tile(const Params &p, int2 tile, int nt, 
                          h * (FMT == MX_FMT_BF16 ? 16 : kLaneBytes);
   const uint8_t *absrow = nullptr;
   float i8_scale = 0.0f;
-  if constexpr (is_nf4(FMT))
+  if constexpr (is_code4(FMT))
     absrow = static_cast<const uint8_t *>(pick(p.wscale, which)) +
              wrow * (p.K / kNf4Block) * absmax_bytes(FMT);
   if constexpr (FMT == MX_FMT_INT8)
@@ -1429,7 +1461,7 @@ __device__ __forceinline__ void stream_tile(const Params &p, int2 tile, int nt, 
 #pragma unroll
     for (int q = 0; q < kQ; ++q)
       c.q[q] = *reinterpret_cast<const u32x4 *>(codes + static_cast<int64_t>(b) * (2 * kLaneBytes) + kPiece * q);
-    c.abs = is_nf4(FMT) ? load_absmax<FMT>(absrow, 2 * b + h) : 0u;
+    c.abs = is_code4(FMT) ? load_absmax<FMT>(absrow, 2 * b + h) : 0u;
   };
 
   f32x16 acc[MB];
@@ -1469,7 +1501,7 @@ __device__ __forceinline__ void stream_tile(const Params &p, int2 tile, int nt, 
     // the absmax values (abs0, abs1), and each table is built when its block
     // begins.
     constexpr bool kSwapTables = MB <= 2;
-    constexpr int kGroup = is_nf4(FMT) ? 1 : 2;  // dwords per group of 8 weights
+    constexpr int kGroup = is_code4(FMT) ? 1 : 2;  // dwords per group of 8 weights
     uint32_t w[4 * kQ];
 #pragma unroll
     for (int q = 0; q < 4 * kQ; ++q) w[q] = cc.q[q >> 2][q & 3];
@@ -1480,6 +1512,9 @@ __device__ __forceinline__ void stream_tile(const Params &p, int2 tile, int nt, 
 #pragma unroll
         for (int q = 0; q < kGroup; ++q) swap_halves(w[kGroup * g + q], w[kGroup * (g + 1) + q]);
     }
+    // MXFP4: the two scales of block 0 and of block 1, in both halves.
+    uint32_t mx0 = cc.abs, mx1 = cc.abs;
+    if constexpr (is_mx4(FMT)) swap_halves(mx0, mx1);
     Nf4Table t0 = {}, t1 = {};
     if constexpr (is_nf4(FMT)) {
       float av;
@@ -1519,7 +1554,9 @@ __device__ __forceinline__ void stream_tile(const Params &p, int2 tile, int nt, 
       // Group of MFMA step s: the even ones of block 0, then the odd ones.
       const int g = BLOCKWISE ? s : 2 * (s & 3) + (s >> 2);
       uint32_t d[4];
-      if constexpr (is_nf4(FMT)) {
+      if constexpr (is_mx4(FMT)) {
+        mx4_decode8(w[g], mx4_scale(s < SUB / 2 ? mx0 : mx1, (s >> 1) & 1), d);
+      } else if constexpr (is_nf4(FMT)) {
         nf4_decode8(t, w[g], d);
       } else if constexpr (FMT == MX_FMT_INT8) {
 #pragma unroll
@@ -1955,6 +1992,8 @@ int launch_tile(int fmt, const Params &p, int64_t max_tiles, hipStream_t s) {
       return launch<MX_FMT_NF4_DQ_KN, EPI, LORA, Short>(p, max_tiles, s);
     case MX_FMT_INT8:
       return launch<MX_FMT_INT8, EPI, LORA, Short>(p, max_tiles, s);
+    case MX_FMT_MXFP4:
+      return launch<MX_FMT_MXFP4, EPI, LORA, Short>(p, max_tiles, s);
     case MX_FMT_F32X3:
       if constexpr (EPI == EPI_SWIGLU || EPI == EPI_STORE)
         return launch<MX_FMT_F32X3, EPI, LORA, Short>(p, max_tiles, s);
@@ -1988,6 +2027,8 @@ int launch_tile_dual(int fmt, const Params &p, int64_t max_tall, int64_t max_sho
       break;
     case MX_FMT_INT8:
       return launch_dual<MX_FMT_INT8, EPI, LORA, Tall, Short>(p, max_tall, max_short, s);
+    case MX_FMT_MXFP4:
+      return launch_dual<MX_FMT_MXFP4, EPI, LORA, Tall, Short>(p, max_tall, max_short, s);
     case MX_FMT_F32X3:
       if constexpr (EPI == EPI_SWIGLU || EPI == EPI_STORE)
         return launch_dual<MX_FMT_F32X3, EPI, LORA, Tall, Short>(p, max_tall, max_short, s);
@@ -2010,6 +2051,8 @@ int launch_stream_fmt(int fmt, const Params &p, int64_t max_tiles, hipStream_t s
       return launch_stream<MX_FMT_NF4_DQ, EPI, LORA>(p, max_tiles, s);
     case MX_FMT_INT8:
       return launch_stream<MX_FMT_INT8, EPI, LORA>(p, max_tiles, s);
+    case MX_FMT_MXFP4:
+      return launch_stream<MX_FMT_MXFP4, EPI, LORA>(p, max_tiles, s);
   }
   set_error("unknown weight format %d", fmt);
   return MX_ERR_INVALID;
@@ -2182,7 +2225,7 @@ int check_weight(const char *name, const char *key, const mx_weight *w, int64_t 
               static_cast<long long>(out_f), static_cast<long long>(in_f));
     return MX_ERR_INVALID;
   }
-  if (w->format < MX_FMT_BF16 || w->format > MX_FMT_NF4_DQ_KN) {
+  if (w->format < MX_FMT_BF16 || w->format > MX_FMT_MXFP4) {
     set_error("%s: weight %s has unknown format %d", name, key, w->format);
     return MX_ERR_INVALID;
   }

@@ -45,6 +45,7 @@ _TWO_LEVEL_BUFFERS = (("_nf4_nabsmax", "nested_absmax"), ("_nf4_offset", "offset
 _BUFFER_SUFFIXES = {
     "nf4": ("_nf4", "_nf4_absmax"),
     "int8": ("_int8", "_scale"),
+    "mxfp4": ("_mxfp4", "_mxfp4_scale"),
     "bf16": ("_bf16", None),
     "fp32": ("_f32x3", None),
 }
@@ -231,6 +232,28 @@ class CompressedGroupedExperts(nn.Module):
             self._two_level.discard(key)
         self._shapes[key] = packed_w.shape
         self._layouts[key] = packed_w.layout
+        self._loaded_dense_keys.add(key)
+
+    def load_packed_mxfp4(self, key: str, *, codes: torch.Tensor, scales: torch.Tensor,
+                          shape: tuple[int, int, int]) -> None:
+        """Adopt MXFP4 blocks of expert tensor ``key`` without re-quantising
+        (quant.from_mxfp4_blocks): e2m1 codes, two to a byte, and the biased
+        exponents of their blocks of 32. ``shape`` is the logical [E, out, in]."""
+        if self._quant_format != "mxfp4":
+            raise ValueError("packed MXFP4 blocks load into a module with quant_format='mxfp4'.")
+        if key not in self._spec.tensor_names:
+            raise ValueError(f"Unknown compressed_weights grouped expert tensor '{key}'.")
+        if int(shape[0]) != self.num_experts:
+            raise ValueError(
+                f"compressed_weights grouped expert tensor {key} has {int(shape[0])} experts, "
+                f"expected {self.num_experts}.")
+        packed = quant.from_mxfp4_blocks(codes=codes, scales=scales,
+                                         shape=tuple(int(v) for v in shape))
+        data_suffix, scale_suffix = _BUFFER_SUFFIXES["mxfp4"]
+        self._set_buffer(f"{key}{data_suffix}", packed.data)
+        self._set_buffer(f"{key}{scale_suffix}", packed.scale)
+        self._shapes[key] = packed.shape
+        self._layouts[key] = packed.layout
         self._loaded_dense_keys.add(key)
 
     def load_bnb_state_dict(self, state: dict, shapes: dict, *, prefix: str = "",
@@ -477,14 +500,23 @@ class CompressedGroupedExperts(nn.Module):
         the same computation as run_for_loop."""
         return self.run_for_loop(tokens, counts)
 
-    def grouped_linear(self, key: str, x: torch.Tensor, *, offsets: torch.Tensor) -> torch.Tensor:
+    def grouped_linear(self, key: str, x: torch.Tensor, *, offsets: torch.Tensor,
+                       activations: str = "bf16") -> torch.Tensor:
         """One projection over expert-sorted rows with inclusive int32 ``offsets``
-        (experts.py:803-827); no per-call group-count cap."""
+        (experts.py:803-827); no per-call group-count cap.
+
+        ``activations="mxfp4"`` (quant_format "mxfp4", no adapter on ``key``)
+        quantises the rows to MXFP4 too and multiplies both operands in 4 bits on
+        the scaled matrix instructions, fp32 sums; the result has x's dtype. The
+        gradient of x is then that of the product with bf16 rows (the rows'
+        quantisation is passed through)."""
+        if activations not in ("bf16", "mxfp4"):
+            raise ValueError("activations must be 'bf16' or 'mxfp4'.")
         if self.prefers_for_loop():
             raise RuntimeError(
                 "Grouped compressed_weights execution requires resident full_dequant expert weights.")
         from .fused import grouped_projection
-        return grouped_projection(self, str(key), x, offsets)
+        return grouped_projection(self, str(key), x, offsets, activations)
 
     def extra_repr(self) -> str:
         return (f"num_experts={self.num_experts}, dtype={self._quant_format}, "

@@ -647,9 +647,96 @@ class _GroupedLinear(torch.autograd.Function):
         return (None, None, *grads)
 
 
-def grouped_projection(module, key, x, offsets):
+def _mxfp4_grouped_forward(module, key, x, offsets):
+    """x [S, in] and the weight both in MXFP4 (mx_mxfp4_grouped_linear)."""
+    device = nat.require_gpu(x)
+    nat.poll_route_errors()
+    packed = module.packed_weight(key)
+    if packed.data.device != device:
+        raise ValueError(f"expert weights live on {packed.data.device}, activations on {device}; "
+                         "move the module with .to(device)")
+    _, out_f, in_f = packed.shape
+    if x.ndim != 2 or int(x.shape[1]) != in_f:
+        raise ValueError(f"x has shape {tuple(x.shape)}, weight '{key}' expects [rows, {in_f}].")
+    if not x.is_floating_point():
+        raise ValueError(f"x must be floating point, got {x.dtype}.")
+    if int(offsets.numel()) != module.num_experts:
+        raise ValueError("offsets must hold one inclusive row end per expert.")
+    offs = offsets.detach()
+    if offs.dtype not in (torch.int32, torch.int64) or offs.device != device:
+        offs = offs.to(device=device, dtype=torch.int64)
+    offs = offs.contiguous()
+    rows = x.detach()
+    if rows.dtype not in (torch.bfloat16, torch.float32):
+        rows = rows.float()
+    rows = rows.contiguous()
+    S = int(rows.shape[0])
+    out = torch.empty((S, out_f), dtype=rows.dtype, device=device)
+    if S == 0:
+        return out.to(x.dtype)
+    lib = nat.load_library()
+    ws = nat.workspace(lib.mx_mxfp4_grouped_linear_workspace_size(S, module.num_experts, in_f),
+                       device)
+    slot = nat.open_error_slot()
+    code = nat.dtype_code(rows.dtype)
+    try:
+        with nat.on_device(device):
+            nat.call("mx_mxfp4_grouped_linear", rows.data_ptr(), code, offs.data_ptr(),
+                     int(offs.dtype == torch.int64), S, module.num_experts, packed.descriptor(),
+                     out.data_ptr(), code, ws.data_ptr(), None if slot is None else slot[1],
+                     nat.stream(device))
+    except BaseException:
+        nat.drop_error_slot(slot, device)
+        raise
+    nat.watch_error_slot(slot, device, "a grouped_linear call")
+    return out if out.dtype == x.dtype else out.to(x.dtype)
+
+
+class _MxGroupedLinear(torch.autograd.Function):
+    """The product of two MXFP4 operands with the gradient of the rows: dX = dY W
+    through the decoded weight, the rows' quantisation passed through."""
+
+    @staticmethod
+    def forward(ctx, module, key, x, offsets):
+        ctx.module, ctx.key, ctx.x_dtype = module, key, x.dtype
+        ctx.save_for_backward(offsets)
+        return _mxfp4_grouped_forward(module, key, x, offsets)
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        module, key = ctx.module, ctx.key
+        (offsets,) = ctx.saved_tensors
+        device = grad_out.device
+        offs = offsets.to(device=device, dtype=torch.int64)
+        counts = torch.diff(offs, prepend=offs.new_zeros(1)).contiguous()
+        packed = module.packed_weight(key)
+        _, out_f, in_f = packed.shape
+        g = grad_out.detach().to(torch.bfloat16).contiguous()
+        S, E = int(g.shape[0]), module.num_experts
+        grad_x = torch.empty((S, in_f), dtype=torch.bfloat16, device=device)
+        lib = nat.load_library()
+        ws = nat.workspace(lib.mx_grouped_linear_backward_workspace_size(S, E, in_f, out_f, 0),
+                           device)
+        # Without adapters the entry point reads no x: any address stands for it.
+        with nat.on_device(device):
+            nat.call("mx_grouped_linear_backward", g.data_ptr(), g.data_ptr(), counts.data_ptr(), S,
+                     E, packed.descriptor(), nat.MxLora(None, None, 0, 0.0), grad_x.data_ptr(), None,
+                     None, ws.data_ptr(), nat.stream(device))
+        return None, None, grad_x.to(ctx.x_dtype), None
+
+
+def grouped_projection(module, key, x, offsets, activations="bf16"):
     """x [S, in] rows grouped by expert with inclusive int32 offsets -> [S, out],
     with autograd to x and the LoRA factors when either requires a gradient."""
+    if activations == "mxfp4":
+        if module.quant_format != "mxfp4":
+            raise ValueError("activations='mxfp4' multiplies weights of quant_format 'mxfp4', not "
+                             f"'{module.quant_format}'.")
+        if key in module.expert_lora:
+            raise ValueError(f"'{key}' carries an adapter, which runs with activations='bf16'.")
+        if torch.is_grad_enabled() and x.requires_grad:
+            return _MxGroupedLinear.apply(module, key, x, offsets)
+        return _mxfp4_grouped_forward(module, key, x, offsets)
     adapter = module.expert_lora[key] if key in module.expert_lora else None
     params = [] if adapter is None else [adapter.lora_a, adapter.lora_b]
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params)):

@@ -7,6 +7,10 @@
              ``from_bnb_nf4`` keeps the same codes with an fp32 absmax
              (kernel format MX_FMT_NF4_F32).
 * ``int8`` : int8 [E, out, in] and bf16 per-output-row scale [E, out].
+* ``mxfp4``: OCP microscaled 4-bit floats: e2m1 codes uint8 [E, out, in/2]
+             (element 2 i in the low nibble of byte i) and one power of two per 32
+             elements, as its biased exponent uint8 [E, out, in/32]. Quantised
+             from the given bf16 or fp32 values (no rounding to bf16 before).
 * ``bf16`` : unquantised bf16 [E, out, in].
 * ``fp32`` : unquantised fp32 as bf16 planes [E, out, 3*in] = [hi | lo | hi]
              (hi = bf16(w), lo = bf16(w - hi)); with fp32 tokens split as
@@ -26,11 +30,12 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _native as nat
+from .mxfp4 import MXFP4Tensor, mxfp4_dequantize, mxfp4_quantize
 
 NF4_BLOCKSIZE = 64
-QUANT_FORMATS = ("nf4", "int8", "bf16", "fp32")
+QUANT_FORMATS = ("nf4", "int8", "mxfp4", "bf16", "fp32")
 _FORMAT_CODES = {"bf16": nat.FMT_BF16, "nf4": nat.FMT_NF4, "int8": nat.FMT_INT8,
-                 "fp32": nat.FMT_F32X3}
+                 "fp32": nat.FMT_F32X3, "mxfp4": nat.FMT_MXFP4}
 
 
 def normalize_quant_format(value: str | None) -> str:
@@ -132,6 +137,9 @@ def quantize(source: torch.Tensor, fmt: str) -> PackedWeight:
         nat.call("mx_nf4_quantize", w.data_ptr(), nat.dtype_code(w.dtype), rows, in_f,
                  codes.data_ptr(), absmax.data_ptr(), s)
         return PackedWeight("nf4", codes, absmax, (E, out_f, in_f))
+    if fmt == "mxfp4":
+        q4 = mxfp4_quantize(w)
+        return PackedWeight("mxfp4", q4.codes, q4.scales, (E, out_f, in_f))
     q = torch.empty((E, out_f, in_f), dtype=torch.int8, device=device)
     scale = torch.empty((E, out_f), dtype=torch.bfloat16, device=device)
     nat.call("mx_int8_quantize", w.data_ptr(), nat.dtype_code(w.dtype), rows, in_f,
@@ -153,6 +161,8 @@ def dequantize(packed: PackedWeight, *, dtype: torch.dtype = torch.bfloat16,
         return (data[..., :in_f].float() + data[..., in_f:2 * in_f].float()).to(dtype)
     nat.require_gpu(data)
     scale_all = packed.scale
+    if packed.fmt == "mxfp4":
+        return mxfp4_dequantize(MXFP4Tensor(data, scale_all[sel], in_f), dtype=dtype)
     if packed.dq is not None:
         # The two-level absmax as the GEMMs decode it, then the fp32-absmax path.
         scale_all = torch.empty((E, *packed.scale.shape[1:]), dtype=torch.float32, device=device)
@@ -180,6 +190,31 @@ def dequantize(packed: PackedWeight, *, dtype: torch.dtype = torch.bfloat16,
         nat.call("mx_int8_dequantize", data.data_ptr(), scale.data_ptr(), rows, in_f,
                  out.data_ptr(), nat.dtype_code(dtype), s)
     return out
+
+
+def from_mxfp4_blocks(*, codes: torch.Tensor, scales: torch.Tensor,
+                      shape: tuple[int, int, int]) -> PackedWeight:
+    """Adopt an MXFP4 expert stack as stored elsewhere, without re-quantising.
+
+    ``codes`` holds E * out * in / 2 bytes in row order, element 2 i of a row in the
+    low nibble of its byte i; ``scales`` E * out * in / 32 biased exponents. Any
+    arrangement of those bytes into dimensions ([E, out, in/32, 16], ...) is taken.
+    """
+    E, out_f, in_f = (int(v) for v in shape)
+    if in_f <= 0 or in_f % 64:
+        raise ValueError(f"in_features must be a multiple of 64 for the MI355X kernels, got {in_f}.")
+    device = nat.require_gpu(codes)
+    for name, t, numel in (("codes", codes, E * out_f * in_f // 2),
+                           ("scales", scales, E * out_f * in_f // 32)):
+        if int(t.numel()) != numel or t.dtype != torch.uint8:
+            raise ValueError(f"MXFP4 {name} must hold {numel} uint8 values, got {int(t.numel())} "
+                             f"{t.dtype}.")
+    # Copies: the weight must not change with the caller's buffers, and the kernels
+    # read 16 bytes at a time.
+    return PackedWeight("mxfp4", codes.detach().reshape(E, out_f, in_f // 2).clone(
+        memory_format=torch.contiguous_format),
+        scales.detach().to(device).reshape(E, out_f, in_f // 32).clone(
+            memory_format=torch.contiguous_format), (E, out_f, in_f))
 
 
 def from_bnb_nf4(*, packed: torch.Tensor, absmax: torch.Tensor, nested_absmax: torch.Tensor,
