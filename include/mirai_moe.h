@@ -25,8 +25,9 @@
  *                   code table), decoded inside the GEMMs
  *   NF4_DQ_KN       NF4_DQ for a weight stored [E, in, out] (as NF4_F32_KN)
  *   MXFP4 weight    codes [E, out, in/2] uint8 (e2m1, element 2 i of a row in the
- *                   low nibble of byte i), `scale` uint8 [E, out, in/32]: the
- *                   biased exponent of the power of two of 32 elements (255: NaN)
+ *                   low nibble of byte i), `scale` uint8 [E, ceil(in/128), out, 4]:
+ *                   the biased exponents (255: NaN) of the powers of two of a row's
+ *                   blocks of 32, those of 128 columns together, zeros past in
  *   NF4_F32_KN      the same codes and fp32 absmax for a weight stored
  *                   [E, in, out] (y = x @ W[e], the MAGI-2 group layout of
  *                   magi2_preview.py:2680-2704): codes [E, in, out/2] packed

@@ -49,7 +49,14 @@ constexpr bool is_nf4(int fmt) {
 }
 // OCP microscaled 4-bit floats: e2m1 codes, element 2 i of a row in the low nibble
 // of byte i, and one power of two (its biased exponent, a byte) per 32 columns.
+// The scales lie as [E][ceil(cols / 128)][rows][4], so that those of neighbouring
+// rows are neighbours.
 constexpr bool is_mx4(int fmt) { return fmt == MX_FMT_MXFP4; }
+// The 4 scales of 128 columns from column block `tile` of 128 on of an expert's row.
+__device__ __forceinline__ const uint8_t *mx4_scales(const void *scale, int64_t e, int64_t cols, int64_t rows,
+                                                     int64_t tile, int64_t row) {
+  return static_cast<const uint8_t *>(scale) + ((e * ((cols + 127) / 128) + tile) * rows + row) * 4;
+}
 // Formats of two codes per byte.
 constexpr bool is_code4(int fmt) { return is_nf4(fmt) || is_mx4(fmt); }
 constexpr bool f32_absmax(int fmt) { return fmt == MX_FMT_NF4_F32 || fmt == MX_FMT_NF4_F32_KN; }
@@ -530,8 +537,9 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
     const uint8_t *w = static_cast<const uint8_t *>(pick(p.w, which));
     if (is_code4(FMT)) {
       b_base = w + wrow * (row_k / 2) + bh * (T::B_ELEMS / 2);
-      b_absmax = static_cast<const uint8_t *>(pick(p.wscale, which)) +
-                 wrow * (row_k / kNf4Block) * absmax_bytes(FMT);
+      b_absmax = is_mx4(FMT) ? mx4_scales(pick(p.wscale, which), e, row_k, wn_rows, 0, bn)
+                             : static_cast<const uint8_t *>(pick(p.wscale, which)) +
+                                   wrow * (row_k / kNf4Block) * absmax_bytes(FMT);
       if (kSplitK && p.k_split < p.K) {
         const int64_t wrow1 = static_cast<int64_t>(e) * p.wn[1] + bn;
         b_base1 = static_cast<const uint8_t *>(p.w[1]) + wrow1 * (row_k / 2) + bh * (T::B_ELEMS / 2);
@@ -605,7 +613,7 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
       if (is_mx4(FMT)) {
         // The lane's 32 columns are one block.
         rb.q[0] = *reinterpret_cast<const u32x4 *>(w + wrow * (p.N / 2) + t_col0 / 2);
-        rb.abs = static_cast<const uint8_t *>(ws)[wrow * (p.N / 32) + t_col0 / 32];
+        rb.abs = mx4_scales(ws, e, p.N, second ? p.wn[1] : p.wn[0], t_col0 / 128, krow)[(t_col0 / 32) & 3];
       } else if (is_nf4(FMT)) {
         rb.q[0] = *reinterpret_cast<const u32x4 *>(w + wrow * (p.N / 2) + t_col0 / 2);
         rb.abs = load_absmax<FMT>(ws, wrow * (p.N / kNf4Block) + t_col0 / kNf4Block);
@@ -638,7 +646,9 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
 #pragma unroll
       for (int q = 0; q < kBRegs; ++q)
         rb.q[q] = *reinterpret_cast<const u32x4 *>(bb + static_cast<int64_t>(ks) * kBStageBytes + 16 * q);
-      rb.abs = is_code4(FMT) ? load_absmax<FMT>(ba, ks * BK / kNf4Block) : 0u;
+      rb.abs = is_mx4(FMT)   ? load_absmax<FMT>(ba, (ks >> 1) * 2 * wn_rows + (ks & 1))
+               : is_nf4(FMT) ? load_absmax<FMT>(ba, ks * BK / kNf4Block)
+                             : 0u;
     } else {
 #pragma unroll
       for (int q = 0; q < kBRegs; ++q) rb.q[q] = u32x4{0u, 0u, 0u, 0u};
@@ -1438,8 +1448,9 @@ __device__ __forceinline__ void stream_tile(const Params &p, int2 tile, int nt, 
   const uint8_t *absrow = nullptr;
   float i8_scale = 0.0f;
   if constexpr (is_code4(FMT))
-    absrow = static_cast<const uint8_t *>(pick(p.wscale, which)) +
-             wrow * (p.K / kNf4Block) * absmax_bytes(FMT);
+    absrow = is_mx4(FMT) ? mx4_scales(pick(p.wscale, which), e, p.K, pick(p.wn, which), 0, n_row)
+                         : static_cast<const uint8_t *>(pick(p.wscale, which)) +
+                               wrow * (p.K / kNf4Block) * absmax_bytes(FMT);
   if constexpr (FMT == MX_FMT_INT8)
     i8_scale = bf16_bits_to_f32(static_cast<const uint16_t *>(pick(p.wscale, which))[wrow]);
   // NF4_DQ: the row's nested scales (K <= 16384: at most two groups).
@@ -1461,7 +1472,9 @@ __device__ __forceinline__ void stream_tile(const Params &p, int2 tile, int nt, 
 #pragma unroll
     for (int q = 0; q < kQ; ++q)
       c.q[q] = *reinterpret_cast<const u32x4 *>(codes + static_cast<int64_t>(b) * (2 * kLaneBytes) + kPiece * q);
-    c.abs = is_code4(FMT) ? load_absmax<FMT>(absrow, 2 * b + h) : 0u;
+    c.abs = is_mx4(FMT)   ? load_absmax<FMT>(absrow, b * 2 * pick(p.wn, which) + h)
+            : is_nf4(FMT) ? load_absmax<FMT>(absrow, 2 * b + h)
+                          : 0u;
   };
 
   f32x16 acc[MB];

@@ -4,6 +4,7 @@
 #include "mxfp4.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mx {
 namespace mxfp4 {
@@ -12,11 +13,12 @@ namespace {
 constexpr int kUnroll = 4;  // groups of 8 elements per thread
 
 // Groups of 8 elements in order of (row, group of the row): four consecutive ones
-// are a block and meet in a quad of lanes.
-template <bool BF16>
+// are a block and meet in a quad of lanes. Scales lie by row or, TILED, as the
+// product reads them: [ceil(cols / 128)][rows][4], zeros past the row's blocks.
+template <bool BF16, bool TILED>
 __device__ __forceinline__ void quantize_groups(const void *x, int64_t rows, int64_t cols,
                                                 int64_t ldx, bool vec, uint8_t *codes,
-                                                uint8_t *scales, int64_t lds, int64_t chunk) {
+                                                uint8_t *scales, int64_t chunk) {
   const int64_t per_row = 4 * ((cols + kBlock - 1) / kBlock);
   const int64_t total = rows * per_row;
   const bool flat = vec && ldx == cols && cols % kBlock == 0;
@@ -46,9 +48,22 @@ __device__ __forceinline__ void quantize_groups(const void *x, int64_t rows, int
     if (g >= total) break;
     uint32_t scale;
     reinterpret_cast<uint32_t *>(codes)[g] = quantize8(v[u], scale);
-    if ((g & 3) == 0) {
-      const int64_t b = g >> 2;
-      scales[4 * lds == per_row ? b : b + row_of(g) * (lds - per_row / 4)] = static_cast<uint8_t>(scale);
+    if constexpr (!TILED) {
+      if ((g & 3) == 0) scales[g >> 2] = static_cast<uint8_t>(scale);
+    } else {
+      const int64_t row = row_of(g), b = (g - row * per_row) >> 2;
+      uint8_t *at = scales + ((b >> 2) * rows + row) * 4;
+      if (per_row % 16 == 0) {
+        // The 16 lanes of 4 blocks put their scales together.
+        uint32_t w = scale << (8 * (b & 3));
+        w |= __builtin_amdgcn_mov_dpp(static_cast<int>(w), 0x141, 0xf, 0xf, true);  // mirrored half row
+        w |= __builtin_amdgcn_mov_dpp(static_cast<int>(w), 0x140, 0xf, 0xf, true);  // mirrored row
+        if ((g & 15) == 0) *reinterpret_cast<uint32_t *>(at) = w;
+      } else if ((g & 3) == 0) {
+        at[b & 3] = static_cast<uint8_t>(scale);
+        if (b == (per_row >> 2) - 1)
+          for (int i = (b & 3) + 1; i < 4; ++i) at[i] = 0;
+      }
     }
   }
 }
@@ -57,7 +72,7 @@ template <bool BF16>
 __global__ __launch_bounds__(256) void quantize_kernel(const void *x, int64_t rows, int64_t cols,
                                                        int64_t ldx, bool vec, uint8_t *codes,
                                                        uint8_t *scales) {
-  quantize_groups<BF16>(x, rows, cols, ldx, vec, codes, scales, (cols + kBlock - 1) / kBlock, blockIdx.x);
+  quantize_groups<BF16, false>(x, rows, cols, ldx, vec, codes, scales, blockIdx.x);
 }
 
 // One group of 8 elements per thread and step.
@@ -126,14 +141,16 @@ bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 
 // ---------------------------------------------------------- grouped product
 constexpr int kTall = 256, kShort = 128;  // rows of the product's tiles
-constexpr int kStep = 256;                // K columns of an LDS stage: 128 bytes of codes
+constexpr int kStage = kTall * 64 + 128 * 64 + kTall * 4 + 128 * 4;  // bytes of an LDS stage
+constexpr int kStep = 128;                // K columns of an LDS stage: 64 bytes of codes
 
 // Workspace: a head of 256 bytes (int32 errors, tall tiles, short tiles), the
-// segment ends as the tiles use them, the tile lists, the rows' codes [S, K/2] and
-// scales [S, ldxs].
+// tile lists, the rows' codes [S, K/2] and
+// scales
+// [ceil(K / 128)][S][4].
 struct Layout {
-  int64_t max_tall = 0, max_short = 0, ldxs = 0;
-  size_t off_ends = 0, off_tall = 0, off_short = 0, off_codes = 0, off_scales = 0, bytes = 0;
+  int64_t max_tall = 0, max_short = 0;
+  size_t off_tall = 0, off_short = 0, off_codes = 0, off_scales = 0, bytes = 0;
 };
 
 Layout layout(int64_t rows, int experts, int64_t in_f) {
@@ -141,18 +158,15 @@ Layout layout(int64_t rows, int experts, int64_t in_f) {
   // A tall tile has more than kShort rows of its expert, a short one at least one.
   L.max_tall = rows / (kShort + 1);
   L.max_short = std::min<int64_t>(rows, experts);
-  L.ldxs = ceil_div(in_f, kStep) * (kStep / kBlock);
   size_t off = 256;
-  L.off_ends = off;
-  off = align_up(off + sizeof(int64_t) * experts, 256);
   L.off_tall = off;
-  off = align_up(off + sizeof(int2) * L.max_tall, 256);
+  off = align_up(off + sizeof(int4) * L.max_tall, 256);
   L.off_short = off;
-  off = align_up(off + sizeof(int2) * L.max_short, 256);
+  off = align_up(off + sizeof(int4) * L.max_short, 256);
   L.off_codes = off;
   off = align_up(off + rows * (in_f / 2), 256);
   L.off_scales = off;
-  off = align_up(off + rows * L.ldxs, 256);
+  off = align_up(off + ceil_div(in_f, kStep) * rows * 4, 256);
   L.bytes = off;
   return L;
 }
@@ -163,8 +177,7 @@ struct PlanOut {
   int64_t rows;
   int experts;
   int32_t *head;  // errors, tall tiles, short tiles
-  int64_t *ends;
-  int2 *tall, *rest;
+  int4 *tall, *rest;  // (expert, first row, rows, 0)
   int32_t *host_err;
 };
 
@@ -214,7 +227,6 @@ __device__ void plan_tiles(const PlanOut &P) {
   for (int e = e0; e < e1; ++e) {
     const int64_t r = raw(e), end = max(start, held(r));
     bad += r < start || r > P.rows;
-    P.ends[e] = end;
     tiles += tall_of(end - start) + (short_of(end - start) << 32);
     start = end;
   }
@@ -227,9 +239,11 @@ __device__ void plan_tiles(const PlanOut &P) {
     const int64_t end = max(start, held(raw(e)));
     int64_t n = tall_of(end - start);
     for (int64_t i = 0; i < n; ++i)
-      P.tall[(at & 0xffffffff) + i] = int2{e, static_cast<int>(start + i * kTall)};
+      P.tall[(at & 0xffffffff) + i] = int4{e, static_cast<int>(start + i * kTall),
+                                           static_cast<int>(min(end - start - i * kTall, int64_t(kTall))), 0};
     if (short_of(end - start)) {
-      P.rest[at >> 32] = int2{e, static_cast<int>(start + n * kTall)};
+      P.rest[at >> 32] = int4{e, static_cast<int>(start + n * kTall),
+                              static_cast<int>(end - start - n * kTall), 0};
       at += int64_t(1) << 32;
     }
     at += n;
@@ -247,23 +261,22 @@ __device__ void plan_tiles(const PlanOut &P) {
 // The rows' quantisation; the last workgroup forms the tile list meanwhile.
 template <bool BF16>
 __global__ __launch_bounds__(256) void rows_kernel(const void *x, int64_t rows, int64_t cols, bool vec,
-                                                   uint8_t *codes, uint8_t *scales, int64_t lds,
-                                                   PlanOut P) {
+                                                   uint8_t *codes, uint8_t *scales, PlanOut P) {
   if (blockIdx.x == gridDim.x - 1) {
     plan_tiles(P);
     return;
   }
-  quantize_groups<BF16>(x, rows, cols, cols, vec, codes, scales, lds, blockIdx.x);
+  // A run of rows per XCD, so that a line of their scales is written by one L2.
+  const int64_t per = gridDim.x >> 3;
+  quantize_groups<BF16, true>(x, rows, cols, cols, vec, codes, scales, (blockIdx.x & 7) * per + (blockIdx.x >> 3));
 }
 
 struct Product {
-  const uint8_t *xc, *xs;  // [S, K/2], [S, ldxs]
-  int64_t ldxs;
-  const uint8_t *wc, *ws;  // [E, N, K/2], [E, N, K/32]
-  int64_t K, N;
+  const uint8_t *xc, *xs;  // [S, K/2], [ceil(K/128)][S][4]
+  const uint8_t *wc, *ws;  // [E, N, K/2], [E, ceil(K/128), N, 4]
+  int64_t S, K, N;
   const int32_t *head;
-  const int64_t *ends;
-  const int2 *tall, *rest;
+  const int4 *tall, *rest;
   int n_tiles_n;
   void *out;
 };
@@ -271,12 +284,8 @@ struct Product {
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// Row key of a stage of 128-byte rows: the 16-byte chunks of 16 consecutive rows at
-// one logical chunk lie in 16 different slots of a 256-byte bank line.
-__device__ __forceinline__ int row_key(int row) { return ((row >> 1) ^ (row << 2)) & 7; }
-
-__device__ __forceinline__ i32x8 fragment(const uint8_t *stage, int row, int chunk) {
-  const u32x4 q = *reinterpret_cast<const u32x4 *>(stage + row * 128 + ((chunk ^ row_key(row)) << 4));
+// 4-bit operands take the first four of the eight registers.
+__device__ __forceinline__ i32x8 operand(u32x4 q) {
   return i32x8{static_cast<int>(q[0]), static_cast<int>(q[1]), static_cast<int>(q[2]),
                static_cast<int>(q[3]), 0, 0, 0, 0};
 }
@@ -287,75 +296,64 @@ __device__ __forceinline__ void lds_dma16(const uint8_t *src, uint8_t *dst) {
       reinterpret_cast<__attribute__((address_space(3))) void *>(reinterpret_cast<uintptr_t>(dst)), 16, 0, 0);
 }
 
-// One tile of up to BM rows x BN weight rows: 4 waves on a WGM x (4 / WGM) grid, each
-// with MB x NB blocks of 32 x 32 (v_mfma_scale_f32_32x32x64_f8f6f4, the weights
-// first: a lane's 4 consecutive values are 4 columns of an output row). K runs in
-// stages of 256 columns through LDS, two stages, filled by DMA.
-template <bool BF16, int BM, int BN, int WGM>
-__device__ __forceinline__ void product_tile(const Product &p, int2 tile, int64_t n0, uint8_t *sX0, uint8_t *sX1,
-                                             uint8_t *sW0, uint8_t *sW1) {
-  constexpr int WGN = 4 / WGM, WM = BM / WGM, WN = BN / WGN, MB = WM / 32, NB = WN / 32;
-  constexpr int XD = BM / 32, WD = BN / 32;  // DMA instructions of a wave per stage
+__device__ __forceinline__ void lds_dma4(const uint8_t *src, uint8_t *dst) {
+  __builtin_amdgcn_global_load_lds(
+      reinterpret_cast<const void *>(src),
+      reinterpret_cast<__attribute__((address_space(3))) void *>(reinterpret_cast<uintptr_t>(dst)), 4, 0, 0);
+}
+
+// A tile of up to 64 MB rows of an expert by 128 of its weight rows, by 4 waves with
+// 32 MB x 64 outputs each: MB x 2 blocks of v_mfma_scale_f32_32x32x64_f8f6f4, the
+// weights first (a lane's 4 consecutive values are 4 columns of an output row).
+// K runs in stages of 128 columns (64 bytes of a row) through a ring of three in
+// LDS, codes and scales filled by DMA two stages ahead: 76.5 KB, so two workgroups
+// share a CU and cover each other's ends. (Scales read from memory by row, a line
+// per row, cost more time in the address units than everything else: 131072 rows,
+// 2048 -> 1408, 64 experts 462 us instead of TODO.)
+template <bool BF16, int MB>
+__device__ __forceinline__ void product_tile(const Product &p, int4 tile, int64_t n0, uint8_t *s0, uint8_t *s1,
+                                             uint8_t *s2) {
+  constexpr int NB = 2, WM = 32 * MB, WN = 64, BM = 2 * WM;
+  constexpr int XD = BM / 64, WD = 2;  // DMA instructions of a wave per stage (16 rows each)
+  // The weights' and the scales' places in a stage.
+  constexpr int kW = BM * 64, kXS = kW + 128 * 64, kWS = kXS + BM * 4;
+  static_assert(kWS + 512 <= kStage, "a stage holds the tile's columns");
   const int lane = threadIdx.x & 63, li = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int wm = wave / WGN, wn = wave % WGN;
-  const int e = tile.x;
+  const int wm = wave >> 1, wn = wave & 1;
+  const int e = tile.x, m = tile.z;
   const int64_t row0 = tile.y;
-  const int m = static_cast<int>(min(p.ends[e] - row0, static_cast<int64_t>(BM)));
-  const int n = static_cast<int>(min(p.N - n0, static_cast<int64_t>(BN)));
-  const int kb = static_cast<int>(p.K / 2);         // bytes of a row's codes
-  const int last = static_cast<int>(p.K / kBlock) - 1;  // its last 16-byte chunk
+  const int n = static_cast<int>(min(p.N - n0, int64_t(128)));
+  const int kb = static_cast<int>(p.K / 2), last = static_cast<int>(p.K / kBlock) - 1;
+  const int KT = static_cast<int>((p.K + 127) / 128);
   const uint8_t *xc = p.xc + row0 * kb;
   const uint8_t *wc = p.wc + (e * p.N + n0) * kb;
-  // Rows past the tile's repeat its last one: their products are not stored.
-  int xoff[XD], woff[WD], chunk[2];
+  // 16-byte chunks of a stage's rows lie at chunk ^ (row >> 2 & 3): of 16 consecutive
+  // rows one chunk is in 16 different slots of a 256-byte bank line. Rows past the
+  // tile's repeat its last one and columns past K the last chunk: their products
+  // are not stored, or vanish by their scales.
+  const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+  uint32_t xo[XD], wo[WD];
 #pragma unroll
-  for (int i = 0; i < XD; ++i) xoff[i] = min((wave * XD + i) * 8 + (lane >> 3), m - 1) * kb;
+  for (int i = 0; i < XD; ++i) xo[i] = __umul24(min(16 * (4 * i + wave) + (lane >> 2), m - 1), kb);
 #pragma unroll
-  for (int i = 0; i < WD; ++i) woff[i] = min((wave * WD + i) * 8 + (lane >> 3), n - 1) * kb;
+  for (int i = 0; i < WD; ++i) wo[i] = __umul24(min(16 * (4 * i + wave) + (lane >> 2), n - 1), kb);
+  // Scales: 4 bytes of a stage per row, 64 rows per DMA instruction (where there
+  // are fewer rows than waves, two waves bring the same ones).
+  const uint8_t *xs = p.xs + row0 * 4;
+  const uint8_t *ws = p.ws + (e * KT * p.N + n0) * 4;
+  const int xg = wave & (BM / 64 - 1), wg = wave & 1;
+  const uint32_t xso = 4 * min(64 * xg + lane, m - 1), wso = 4 * min(64 * wg + lane, n - 1);
+  auto load = [&](int k, uint8_t *s) __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t c = 16 * min(4 * k + chunk, last);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) chunk[i] = (lane & 7) ^ row_key(8 * i + (lane >> 3));
-  static_assert(XD % 2 == 0 && WD % 2 == 0, "a DMA's rows begin at an even multiple of 8 for even i");
-  auto load = [&](int k, uint8_t *sX, uint8_t *sW) __attribute__((always_inline)) {
-    // Chunks past K repeat the last one: the steps they belong to are left out.
-    const int c[2] = {16 * min(8 * k + chunk[0], last), 16 * min(8 * k + chunk[1], last)};
+    for (int i = 0; i < XD; ++i) lds_dma16(xc + (xo[i] + c), s + (4 * i + wave) * 1024);
 #pragma unroll
-    for (int i = 0; i < XD; ++i) lds_dma16(xc + (xoff[i] + c[i & 1]), sX + (wave * XD + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < WD; ++i) lds_dma16(wc + (woff[i] + c[i & 1]), sW + (wave * WD + i) * 1024);
-  };
-  // Scales of the wave's rows: the 8 bytes of a stage per lane and block of 32 rows.
-  struct __attribute__((packed, aligned(2))) Eight {
-    uint64_t v;
-  };
-  const uint8_t *xs[MB], *ws[NB];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) xs[mb] = p.xs + (row0 + min(wm * WM + 32 * mb + li, m - 1)) * p.ldxs;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-    ws[nb] = p.ws + (e * p.N + n0 + min(wn * WN + 32 * nb + li, n - 1)) * (p.K / kBlock);
-  const int KT = static_cast<int>((p.K + kStep - 1) / kStep);
-  const int tail = static_cast<int>(p.K % kStep) / 64;  // 64-column steps of a short last stage
-  struct Scales {
-    uint64_t x[MB], w[NB];
-  };
-  auto load_scales = [&](int k, Scales &s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) s.x[mb] = *reinterpret_cast<const uint64_t *>(xs[mb] + 8 * k);
-    if (tail != 0 && k == KT - 1) {
-      // A weight row's scales end with it.
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const uint16_t *q = reinterpret_cast<const uint16_t *>(ws[nb] + 8 * k);
-        uint64_t v = q[0];
-        if (tail > 1) v |= static_cast<uint64_t>(q[1]) << 16;
-        if (tail > 2) v |= static_cast<uint64_t>(q[2]) << 32;
-        s.w[nb] = v;
-      }
-    } else {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) s.w[nb] = reinterpret_cast<const Eight *>(ws[nb] + 8 * k)->v;
-    }
+    for (int i = 0; i < WD; ++i) lds_dma16(wc + (wo[i] + c), s + kW + (4 * i + wave) * 1024);
+    lds_dma4(xs + (4 * k * p.S + xso), s + kXS + 256 * xg);
+    lds_dma4(ws + (4 * k * p.N + wso), s + kWS + 256 * wg);
+    __builtin_amdgcn_sched_barrier(0);
   };
   f32x16 acc[MB][NB];
 #pragma unroll
@@ -363,62 +361,72 @@ __device__ __forceinline__ void product_tile(const Product &p, int2 tile, int64_
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) acc[mb][nb][j] = 0.0f;
-
-  auto step = [&](int k, const uint8_t *sX, const uint8_t *sW, uint8_t *nX, uint8_t *nW, const Scales &cur,
-                  Scales &nxt) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this stage has landed
-    __syncthreads();
-    if (k + 1 < KT) {
-      load(k + 1, nX, nW);
-      load_scales(k + 1, nxt);
+      for (int q = 0; q < 16; ++q) acc[mb][nb][q] = 0.0f;
+  // Half h of a step's 64 columns: chunk 2 s + h, at the first one's place ^ (s << 5).
+  const int place0 = li * 64 + ((h ^ ((li >> 2) & 3)) << 4);
+  const int fx = wm * WM * 64 + place0, fw = kW + wn * WN * 64 + place0;
+  const int sxo = kXS + 4 * (wm * WM + li), swo = kWS + 4 * (wn * WN + li);
+  auto step = [&](int k, const uint8_t *s, uint8_t *refill) __attribute__((always_inline)) {
+    // The stage has landed once only the DMA of the one after it is under way, and
+    // the reads of the one before it, which is refilled, are done (lgkmcnt(0)).
+    if (k + 1 < KT)
+      __builtin_amdgcn_s_waitcnt(0x0070 | (XD + WD + 2));
+    else
+      __builtin_amdgcn_s_waitcnt(0x0070);
+    // (A fence would wait for all of the DMA.)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if (k + 2 < KT) load(k + 2, refill);
+    // Byte 0 of a shifted word: the scale of the lane's block of the first 64 columns;
+    // byte 2: of the second. (Past K they are 2^-127 on both sides: products of at most
+    // 36 * 2^-254, which vanish next to any fp32 number.)
+    int sx[MB], sw[NB];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+      sx[mb] = static_cast<int>(*reinterpret_cast<const uint32_t *>(s + sxo + 128 * mb) >> (8 * h));
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+      sw[nb] = static_cast<int>(*reinterpret_cast<const uint32_t *>(s + swo + 128 * nb) >> (8 * h));
+    u32x4 x[2][MB], w[2][NB];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) w[t][nb] = *reinterpret_cast<const u32x4 *>(s + (fw ^ (t << 5)) + 2048 * nb);
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) x[t][mb] = *reinterpret_cast<const u32x4 *>(s + (fx ^ (t << 5)) + 2048 * mb);
     }
-    const int subs = k == KT - 1 && tail != 0 ? tail : 4;
-    // Byte 0 of a half word pair: the lane's block of its first step; byte 2: of the second.
-    int sx[2][MB], sw[2][NB];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) sx[i][mb] = static_cast<int>(static_cast<uint32_t>(cur.x[mb] >> (32 * i)) >> (8 * h));
+      for (int nb = 0; nb < NB; ++nb)
+        acc[mb][nb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w[0][nb]), operand(x[0][mb]),
+                                                                      acc[mb][nb], 4, 4, 0, sw[nb], 0, sx[mb]);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) sw[i][nb] = static_cast<int>(static_cast<uint32_t>(cur.w[nb] >> (32 * i)) >> (8 * h));
-    }
+    for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if (s >= subs) break;
-      i32x8 x[MB], w[NB];
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) x[mb] = fragment(sX, wm * WM + 32 * mb + li, 2 * s + h);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) w[nb] = fragment(sW, wn * WN + 32 * nb + li, 2 * s + h);
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-          if (s & 1)
-            acc[mb][nb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                w[nb], x[mb], acc[mb][nb], 4, 4, 2, sw[s >> 1][nb], 2, sx[s >> 1][mb]);
-          else
-            acc[mb][nb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                w[nb], x[mb], acc[mb][nb], 4, 4, 0, sw[s >> 1][nb], 0, sx[s >> 1][mb]);
-    }
+      for (int nb = 0; nb < NB; ++nb)
+        acc[mb][nb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w[1][nb]), operand(x[1][mb]),
+                                                                      acc[mb][nb], 4, 4, 2, sw[nb], 2, sx[mb]);
   };
-  Scales s0, s1;
-  load(0, sX0, sW0);
-  load_scales(0, s0);
-  int k = 0;
-  for (; k + 1 < KT; k += 2) {
-    step(k, sX0, sW0, sX1, sW1, s0, s1);
-    step(k + 1, sX1, sW1, sX0, sW0, s1, s0);
+  load(0, s0);
+  if (KT > 1) load(1, s1);
+  for (int k = 0;; k += 3) {
+    step(k, s0, s2);
+    if (k + 1 >= KT) break;
+    step(k + 1, s1, s0);
+    if (k + 2 >= KT) break;
+    step(k + 2, s2, s1);
+    if (k + 3 >= KT) break;
   }
-  if (k < KT) step(k, sX0, sW0, sX1, sW1, s0, s1);
 
-  // Each wave turns 32 rows at a time over in its part of LDS, so that a row's
-  // columns leave in runs of WN values.
+  // Each wave turns 32 rows of its results over at a time in its part of a stage, so
+  // that runs of 64 columns of a row are stored.
   constexpr int ES = BF16 ? 2 : 4, CH = WN * ES / 16;  // 16-byte chunks of a row
   __syncthreads();
-  uint8_t *strip = wave == 0 ? sX0 : wave == 1 ? sX1 : wave == 2 ? sW0 : sW1;
-  auto place = [&](int row, int c) { return row * (CH * 16) + ((c ^ (row & (CH - 1))) << 4); };
+  uint8_t *strip = (wave < 2 ? s0 : s1) + (wave & 1) * 8192;
+  auto place = [&](int row, int c) { return row * (CH * 16) + ((c ^ (BF16 ? (row >> 1) & 7 : row & 15)) << 4); };
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
@@ -438,13 +446,16 @@ __device__ __forceinline__ void product_tile(const Product &p, int2 tile, int64_
       }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    constexpr int RP = 64 / CH, IT = 32 / RP;  // rows per pass, passes
+    u32x4 q[IT];
 #pragma unroll
-    for (int i = 0; i < 32 * CH / 64; ++i) {
-      const int row = (64 * i + lane) / CH, c = lane % CH;
-      const int r = wm * WM + 32 * mb + row, col = wn * WN + c * (16 / ES);
-      const u32x4 q = *reinterpret_cast<const u32x4 *>(strip + place(row, c));
-      if (r < m && col < n)
-        *reinterpret_cast<u32x4 *>(static_cast<uint8_t *>(p.out) + ((row0 + r) * p.N + n0 + col) * ES) = q;
+    for (int i = 0; i < IT; ++i) q[i] = *reinterpret_cast<const u32x4 *>(strip + place(RP * i + lane / CH, lane % CH));
+    const int r0 = wm * WM + 32 * mb + lane / CH, col = wn * WN + (lane % CH) * (16 / ES);
+    uint8_t *out = static_cast<uint8_t *>(p.out) + ((row0 + r0) * p.N + n0 + col) * ES;
+    if (col < n) {
+#pragma unroll
+      for (int i = 0; i < IT; ++i)
+        if (r0 + RP * i < m) *reinterpret_cast<u32x4 *>(out + RP * i * p.N * ES) = q[i];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -455,9 +466,8 @@ __device__ __forceinline__ void product_tile(const Product &p, int2 tile, int64_
 // then a run of the short ones, column tiles of one row tile side by side, so that
 // the rows of a tile and the weights of an expert are read through one L2.
 template <bool BF16>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void product_kernel(Product p) {
-  __shared__ __attribute__((aligned(16))) uint8_t sX0[kTall * 128], sX1[kTall * 128];
-  __shared__ __attribute__((aligned(16))) uint8_t sW0[kTall * 128], sW1[kTall * 128];
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void product_kernel(Product p) {
+  __shared__ __attribute__((aligned(16))) uint8_t s0[kStage], s1[kStage], s2[kStage];
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
   const int total_t = p.head[1] * p.n_tiles_n, total_s = p.head[2] * p.n_tiles_n;
   const int per_t = (total_t + 7) >> 3, per_s = (total_s + 7) >> 3;
@@ -466,20 +476,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   if (!tall && slot >= per_t + per_s) return;
   if (logical >= (tall ? total_t : total_s)) return;
   const int mt = logical / p.n_tiles_n;
-  const int2 tile = (tall ? p.tall : p.rest)[mt];
-  const int64_t n0 = static_cast<int64_t>(logical - mt * p.n_tiles_n) * 256;
-  const bool half = p.N - n0 <= 128;
-  if (tall) {
-    if (half)
-      product_tile<BF16, 256, 128, 2>(p, tile, n0, sX0, sX1, sW0, sW1);
-    else
-      product_tile<BF16, 256, 256, 2>(p, tile, n0, sX0, sX1, sW0, sW1);
-  } else {
-    if (half)
-      product_tile<BF16, 128, 128, 2>(p, tile, n0, sX0, sX1, sW0, sW1);
-    else
-      product_tile<BF16, 128, 256, 2>(p, tile, n0, sX0, sX1, sW0, sW1);
-  }
+  const int4 tile = (tall ? p.tall : p.rest)[mt];
+  const int64_t n0 = static_cast<int64_t>(logical - mt * p.n_tiles_n) * 128;
+  if (tall)
+    product_tile<BF16, 4>(p, tile, n0, s0, s1, s2);
+  else
+    product_tile<BF16, 2>(p, tile, n0, s0, s1, s2);
 }
 
 bool dtype_ok(int d) { return d == MX_DTYPE_BF16 || d == MX_DTYPE_F32; }
@@ -589,19 +591,19 @@ extern "C" int mx_mxfp4_grouped_linear(const void *x, int x_dtype, const void *o
   uint8_t *codes = reinterpret_cast<uint8_t *>(base + L.off_codes);
   uint8_t *scales = reinterpret_cast<uint8_t *>(base + L.off_scales);
   PlanOut P = {offsets, offsets_64 != 0, num_rows, num_experts, reinterpret_cast<int32_t *>(base),
-               reinterpret_cast<int64_t *>(base + L.off_ends), reinterpret_cast<int2 *>(base + L.off_tall),
-               reinterpret_cast<int2 *>(base + L.off_short), host_err};
-  const int64_t chunks = ceil_div(num_rows * (K / 8), 256 * kUnroll);
-  const int64_t n_tiles = ceil_div(N, 256);
+               reinterpret_cast<int4 *>(base + L.off_tall), reinterpret_cast<int4 *>(base + L.off_short),
+               host_err};
+  const int64_t chunks = 8 * ceil_div(ceil_div(num_rows * (K / 8), 256 * kUnroll), 8);
+  const int64_t n_tiles = ceil_div(N, 128);
   const int64_t grid = 8 * (ceil_div(L.max_tall * n_tiles, 8) + ceil_div(L.max_short * n_tiles, 8));
   if (int rc = grid_ok(name, std::max(chunks + 1, grid))) return rc;
   const bool bf16 = x_dtype == MX_DTYPE_BF16;
   auto rows_k = bf16 ? rows_kernel<true> : rows_kernel<false>;
   hipLaunchKernelGGL(rows_k, dim3(static_cast<unsigned>(chunks + 1)), dim3(256), 0, s, x, num_rows, K,
-                     aligned16(x), codes, scales, L.ldxs, P);
+                     aligned16(x), codes, scales, P);
   if (int rc = check_launch(name)) return rc;
-  Product p = {codes, scales, L.ldxs, static_cast<const uint8_t *>(w->data),
-               static_cast<const uint8_t *>(w->scale), K, N, P.head, P.ends, P.tall, P.rest,
+  Product p = {codes, scales, static_cast<const uint8_t *>(w->data),
+               static_cast<const uint8_t *>(w->scale), num_rows, K, N, P.head, P.tall, P.rest,
                static_cast<int>(n_tiles), out};
   auto product = out_dtype == MX_DTYPE_BF16 ? product_kernel<true> : product_kernel<false>;
   hipLaunchKernelGGL(product, dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, p);

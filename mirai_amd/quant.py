@@ -9,8 +9,10 @@
 * ``int8`` : int8 [E, out, in] and bf16 per-output-row scale [E, out].
 * ``mxfp4``: OCP microscaled 4-bit floats: e2m1 codes uint8 [E, out, in/2]
              (element 2 i in the low nibble of byte i) and one power of two per 32
-             elements, as its biased exponent uint8 [E, out, in/32]. Quantised
-             from the given bf16 or fp32 values (no rounding to bf16 before).
+             elements, as its biased exponent, in uint8 [E, ceil(in/128), out, 4]
+             (those of 128 columns together, zeros past in: neighbouring rows'
+             scales are neighbours for the kernels). Quantised from the given bf16
+             or fp32 values (no rounding to bf16 before).
 * ``bf16`` : unquantised bf16 [E, out, in].
 * ``fp32`` : unquantised fp32 as bf16 planes [E, out, 3*in] = [hi | lo | hi]
              (hi = bf16(w), lo = bf16(w - hi)); with fp32 tokens split as
@@ -30,7 +32,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _native as nat
-from .mxfp4 import MXFP4Tensor, mxfp4_dequantize, mxfp4_quantize
+from .mxfp4 import MX_BLOCK, MXFP4Tensor, mxfp4_dequantize, mxfp4_quantize
 
 NF4_BLOCKSIZE = 64
 QUANT_FORMATS = ("nf4", "int8", "mxfp4", "bf16", "fp32")
@@ -139,7 +141,7 @@ def quantize(source: torch.Tensor, fmt: str) -> PackedWeight:
         return PackedWeight("nf4", codes, absmax, (E, out_f, in_f))
     if fmt == "mxfp4":
         q4 = mxfp4_quantize(w)
-        return PackedWeight("mxfp4", q4.codes, q4.scales, (E, out_f, in_f))
+        return PackedWeight("mxfp4", q4.codes, _tile_scales(q4.scales), (E, out_f, in_f))
     q = torch.empty((E, out_f, in_f), dtype=torch.int8, device=device)
     scale = torch.empty((E, out_f), dtype=torch.bfloat16, device=device)
     nat.call("mx_int8_quantize", w.data_ptr(), nat.dtype_code(w.dtype), rows, in_f,
@@ -162,7 +164,8 @@ def dequantize(packed: PackedWeight, *, dtype: torch.dtype = torch.bfloat16,
     nat.require_gpu(data)
     scale_all = packed.scale
     if packed.fmt == "mxfp4":
-        return mxfp4_dequantize(MXFP4Tensor(data, scale_all[sel], in_f), dtype=dtype)
+        rows = scale_all[sel].permute(0, 2, 1, 3).reshape(E, out_f, -1)[..., :in_f // MX_BLOCK]
+        return mxfp4_dequantize(MXFP4Tensor(data, rows, in_f), dtype=dtype)
     if packed.dq is not None:
         # The two-level absmax as the GEMMs decode it, then the fp32-absmax path.
         scale_all = torch.empty((E, *packed.scale.shape[1:]), dtype=torch.float32, device=device)
@@ -209,12 +212,20 @@ def from_mxfp4_blocks(*, codes: torch.Tensor, scales: torch.Tensor,
         if int(t.numel()) != numel or t.dtype != torch.uint8:
             raise ValueError(f"MXFP4 {name} must hold {numel} uint8 values, got {int(t.numel())} "
                              f"{t.dtype}.")
-    # Copies: the weight must not change with the caller's buffers, and the kernels
-    # read 16 bytes at a time.
+    # A copy of the codes: the weight must not change with the caller's buffers, and
+    # the kernels read 16 bytes at a time.
     return PackedWeight("mxfp4", codes.detach().reshape(E, out_f, in_f // 2).clone(
         memory_format=torch.contiguous_format),
-        scales.detach().to(device).reshape(E, out_f, in_f // 32).clone(
-            memory_format=torch.contiguous_format), (E, out_f, in_f))
+        _tile_scales(scales.detach().to(device).reshape(E, out_f, in_f // MX_BLOCK)),
+        (E, out_f, in_f))
+
+
+def _tile_scales(scales: torch.Tensor) -> torch.Tensor:
+    """Row scales [E, out, in/32] -> [E, ceil(in/128), out, 4], zeros past in."""
+    E, out_f, blocks = (int(v) for v in scales.shape)
+    tiles = -(-blocks // 4)
+    padded = torch.nn.functional.pad(scales, (0, 4 * tiles - blocks))
+    return padded.view(E, out_f, tiles, 4).permute(0, 2, 1, 3).contiguous()
 
 
 def from_bnb_nf4(*, packed: torch.Tensor, absmax: torch.Tensor, nested_absmax: torch.Tensor,
