@@ -13,8 +13,9 @@ namespace {
 constexpr int kUnroll = 4;  // groups of 8 elements per thread
 
 // Groups of 8 elements in order of (row, group of the row): four consecutive ones
-// are a block and meet in a quad of lanes. Scales lie by row or, TILED, as the
-// product reads them: [ceil(cols / 128)][rows][4], zeros past the row's blocks.
+// are a block and meet in a quad of lanes. Codes and scales lie by row or, TILED, as
+// the product reads them: [ceil(cols / 128)][rows][64] and [ceil(cols / 128)][rows][4],
+// zeros past the row's blocks.
 template <bool BF16, bool TILED>
 __device__ __forceinline__ void quantize_groups(const void *x, int64_t rows, int64_t cols,
                                                 int64_t ldx, bool vec, uint8_t *codes,
@@ -47,11 +48,14 @@ __device__ __forceinline__ void quantize_groups(const void *x, int64_t rows, int
     const int64_t g = g0 + 256 * u;
     if (g >= total) break;
     uint32_t scale;
-    reinterpret_cast<uint32_t *>(codes)[g] = quantize8(v[u], scale);
+    const uint32_t c = quantize8(v[u], scale);
     if constexpr (!TILED) {
+      reinterpret_cast<uint32_t *>(codes)[g] = c;
       if ((g & 3) == 0) scales[g >> 2] = static_cast<uint8_t>(scale);
     } else {
-      const int64_t row = row_of(g), b = (g - row * per_row) >> 2;
+      const int64_t row = row_of(g), q = g - row * per_row, b = q >> 2;
+      uint32_t *code = reinterpret_cast<uint32_t *>(codes) + ((q >> 4) * rows + row) * 16 + (q & 15);
+      *code = c;
       uint8_t *at = scales + ((b >> 2) * rows + row) * 4;
       if (per_row % 16 == 0) {
         // The 16 lanes of 4 blocks put their scales together.
@@ -64,6 +68,9 @@ __device__ __forceinline__ void quantize_groups(const void *x, int64_t rows, int
         if (b == (per_row >> 2) - 1)
           for (int i = (b & 3) + 1; i < 4; ++i) at[i] = 0;
       }
+      // The row's codes past its last group.
+      if (q == per_row - 1)
+        for (int i = 1; i < 16 - static_cast<int>(q & 15); ++i) code[i] = 0;
     }
   }
 }
@@ -145,7 +152,7 @@ constexpr int kStage = kTall * 64 + 128 * 64 + kTall * 4 + 128 * 4;  // bytes of
 constexpr int kStep = 128;                // K columns of an LDS stage: 64 bytes of codes
 
 // Workspace: a head of 256 bytes (int32 errors, tall tiles, short tiles), the
-// tile lists, the rows' codes [S, K/2] and
+// tile lists, the rows' codes [ceil(K / 128)][S][64] and
 // scales
 // [ceil(K / 128)][S][4].
 struct Layout {
@@ -164,7 +171,7 @@ Layout layout(int64_t rows, int experts, int64_t in_f) {
   L.off_short = off;
   off = align_up(off + sizeof(int4) * L.max_short, 256);
   L.off_codes = off;
-  off = align_up(off + rows * (in_f / 2), 256);
+  off = align_up(off + ceil_div(in_f, kStep) * rows * 64, 256);
   L.off_scales = off;
   off = align_up(off + ceil_div(in_f, kStep) * rows * 4, 256);
   L.bytes = off;
@@ -272,8 +279,8 @@ __global__ __launch_bounds__(256) void rows_kernel(const void *x, int64_t rows, 
 }
 
 struct Product {
-  const uint8_t *xc, *xs;  // [S, K/2], [ceil(K/128)][S][4]
-  const uint8_t *wc, *ws;  // [E, N, K/2], [E, ceil(K/128), N, 4]
+  const uint8_t *xc, *xs;  // [ceil(K/128)][S][64], [ceil(K/128)][S][4]
+  const uint8_t *wc, *ws;  // [E, ceil(K/128), N, 64], [E, ceil(K/128), N, 4]
   int64_t S, K, N;
   const int32_t *head;
   const int4 *tall, *rest;
@@ -305,8 +312,8 @@ __device__ __forceinline__ void lds_dma4(const uint8_t *src, uint8_t *dst) {
 // A tile of up to 64 MB rows of an expert by 128 of its weight rows, by 4 waves with
 // 32 MB x 64 outputs each: MB x 2 blocks of v_mfma_scale_f32_32x32x64_f8f6f4, the
 // weights first (a lane's 4 consecutive values are 4 columns of an output row).
-// K runs in stages of 128 columns (64 bytes of a row) through a ring of three in
-// LDS, codes and scales filled by DMA two stages ahead: 76.5 KB, so two workgroups
+// K runs in stages of 128 columns (64 bytes of a row; rows of a stage side by side
+// in memory, so that requests are of whole lines) through a ring of three in LDS, codes and scales filled by DMA two stages ahead: 76.5 KB, so two workgroups
 // share a CU and cover each other's ends. (Scales read from memory by row, a line
 // per row, cost more time in the address units than everything else: 131072 rows,
 // 2048 -> 1408, 64 experts 462 us instead of TODO.)
@@ -324,20 +331,18 @@ __device__ __forceinline__ void product_tile(const Product &p, int4 tile, int64_
   const int e = tile.x, m = tile.z;
   const int64_t row0 = tile.y;
   const int n = static_cast<int>(min(p.N - n0, int64_t(128)));
-  const int kb = static_cast<int>(p.K / 2), last = static_cast<int>(p.K / kBlock) - 1;
   const int KT = static_cast<int>((p.K + 127) / 128);
-  const uint8_t *xc = p.xc + row0 * kb;
-  const uint8_t *wc = p.wc + (e * p.N + n0) * kb;
+  const uint8_t *xc = p.xc + row0 * 64;
+  const uint8_t *wc = p.wc + (e * KT * p.N + n0) * 64;
   // 16-byte chunks of a stage's rows lie at chunk ^ (row >> 2 & 3): of 16 consecutive
   // rows one chunk is in 16 different slots of a 256-byte bank line. Rows past the
-  // tile's repeat its last one and columns past K the last chunk: their products
-  // are not stored, or vanish by their scales.
-  const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+  // tile's repeat its last one: their products are not stored.
+  const int chunk = 16 * ((lane & 3) ^ ((lane >> 4) & 3));
   uint32_t xo[XD], wo[WD];
 #pragma unroll
-  for (int i = 0; i < XD; ++i) xo[i] = __umul24(min(16 * (4 * i + wave) + (lane >> 2), m - 1), kb);
+  for (int i = 0; i < XD; ++i) xo[i] = 64 * min(16 * (4 * i + wave) + (lane >> 2), m - 1) + chunk;
 #pragma unroll
-  for (int i = 0; i < WD; ++i) wo[i] = __umul24(min(16 * (4 * i + wave) + (lane >> 2), n - 1), kb);
+  for (int i = 0; i < WD; ++i) wo[i] = 64 * min(16 * (4 * i + wave) + (lane >> 2), n - 1) + chunk;
   // Scales: 4 bytes of a stage per row, 64 rows per DMA instruction (where there
   // are fewer rows than waves, two waves bring the same ones).
   const uint8_t *xs = p.xs + row0 * 4;
@@ -346,11 +351,10 @@ __device__ __forceinline__ void product_tile(const Product &p, int4 tile, int64_
   const uint32_t xso = 4 * min(64 * xg + lane, m - 1), wso = 4 * min(64 * wg + lane, n - 1);
   auto load = [&](int k, uint8_t *s) __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
-    const uint32_t c = 16 * min(4 * k + chunk, last);
 #pragma unroll
-    for (int i = 0; i < XD; ++i) lds_dma16(xc + (xo[i] + c), s + (4 * i + wave) * 1024);
+    for (int i = 0; i < XD; ++i) lds_dma16(xc + 64 * k * p.S + xo[i], s + (4 * i + wave) * 1024);
 #pragma unroll
-    for (int i = 0; i < WD; ++i) lds_dma16(wc + (wo[i] + c), s + kW + (4 * i + wave) * 1024);
+    for (int i = 0; i < WD; ++i) lds_dma16(wc + 64 * k * p.N + wo[i], s + kW + (4 * i + wave) * 1024);
     lds_dma4(xs + (4 * k * p.S + xso), s + kXS + 256 * xg);
     lds_dma4(ws + (4 * k * p.N + wso), s + kWS + 256 * wg);
     __builtin_amdgcn_sched_barrier(0);

@@ -7,12 +7,12 @@
              ``from_bnb_nf4`` keeps the same codes with an fp32 absmax
              (kernel format MX_FMT_NF4_F32).
 * ``int8`` : int8 [E, out, in] and bf16 per-output-row scale [E, out].
-* ``mxfp4``: OCP microscaled 4-bit floats: e2m1 codes uint8 [E, out, in/2]
-             (element 2 i in the low nibble of byte i) and one power of two per 32
-             elements, as its biased exponent, in uint8 [E, ceil(in/128), out, 4]
-             (those of 128 columns together, zeros past in: neighbouring rows'
-             scales are neighbours for the kernels). Quantised from the given bf16
-             or fp32 values (no rounding to bf16 before).
+* ``mxfp4``: OCP microscaled 4-bit floats, by 128 columns so that neighbouring
+             rows are neighbours for the kernels: e2m1 codes uint8
+             [E, ceil(in/128), out, 64] (element 2 i of a row in the low nibble of
+             its byte i) and one power of two per 32 elements, as its biased
+             exponent, uint8 [E, ceil(in/128), out, 4]; zeros past in. Quantised
+             from the given bf16 or fp32 values (no rounding to bf16 before).
 * ``bf16`` : unquantised bf16 [E, out, in].
 * ``fp32`` : unquantised fp32 as bf16 planes [E, out, 3*in] = [hi | lo | hi]
              (hi = bf16(w), lo = bf16(w - hi)); with fp32 tokens split as
@@ -141,7 +141,8 @@ def quantize(source: torch.Tensor, fmt: str) -> PackedWeight:
         return PackedWeight("nf4", codes, absmax, (E, out_f, in_f))
     if fmt == "mxfp4":
         q4 = mxfp4_quantize(w)
-        return PackedWeight("mxfp4", q4.codes, _tile_scales(q4.scales), (E, out_f, in_f))
+        return PackedWeight("mxfp4", _by_tiles(q4.codes, 64), _by_tiles(q4.scales, 4),
+                            (E, out_f, in_f))
     q = torch.empty((E, out_f, in_f), dtype=torch.int8, device=device)
     scale = torch.empty((E, out_f), dtype=torch.bfloat16, device=device)
     nat.call("mx_int8_quantize", w.data_ptr(), nat.dtype_code(w.dtype), rows, in_f,
@@ -164,8 +165,9 @@ def dequantize(packed: PackedWeight, *, dtype: torch.dtype = torch.bfloat16,
     nat.require_gpu(data)
     scale_all = packed.scale
     if packed.fmt == "mxfp4":
-        rows = scale_all[sel].permute(0, 2, 1, 3).reshape(E, out_f, -1)[..., :in_f // MX_BLOCK]
-        return mxfp4_dequantize(MXFP4Tensor(data, rows, in_f), dtype=dtype)
+        codes = _by_rows(data, in_f // 2)
+        return mxfp4_dequantize(MXFP4Tensor(codes, _by_rows(scale_all[sel], in_f // MX_BLOCK), in_f),
+                                dtype=dtype)
     if packed.dq is not None:
         # The two-level absmax as the GEMMs decode it, then the fp32-absmax path.
         scale_all = torch.empty((E, *packed.scale.shape[1:]), dtype=torch.float32, device=device)
@@ -212,20 +214,25 @@ def from_mxfp4_blocks(*, codes: torch.Tensor, scales: torch.Tensor,
         if int(t.numel()) != numel or t.dtype != torch.uint8:
             raise ValueError(f"MXFP4 {name} must hold {numel} uint8 values, got {int(t.numel())} "
                              f"{t.dtype}.")
-    # A copy of the codes: the weight must not change with the caller's buffers, and
-    # the kernels read 16 bytes at a time.
-    return PackedWeight("mxfp4", codes.detach().reshape(E, out_f, in_f // 2).clone(
-        memory_format=torch.contiguous_format),
-        _tile_scales(scales.detach().to(device).reshape(E, out_f, in_f // MX_BLOCK)),
+    return PackedWeight(
+        "mxfp4", _by_tiles(codes.detach().reshape(E, out_f, in_f // 2), 64),
+        _by_tiles(scales.detach().to(device).reshape(E, out_f, in_f // MX_BLOCK), 4),
         (E, out_f, in_f))
 
 
-def _tile_scales(scales: torch.Tensor) -> torch.Tensor:
-    """Row scales [E, out, in/32] -> [E, ceil(in/128), out, 4], zeros past in."""
-    E, out_f, blocks = (int(v) for v in scales.shape)
-    tiles = -(-blocks // 4)
-    padded = torch.nn.functional.pad(scales, (0, 4 * tiles - blocks))
-    return padded.view(E, out_f, tiles, 4).permute(0, 2, 1, 3).contiguous()
+def _by_tiles(rows: torch.Tensor, width: int) -> torch.Tensor:
+    """[E, out, n] bytes -> a new [E, ceil(n / width), out, width], zeros past n."""
+    E, out_f, n = (int(v) for v in rows.shape)
+    tiles = -(-n // width)
+    padded = torch.nn.functional.pad(rows, (0, width * tiles - n))
+    return padded.reshape(E, out_f, tiles, width).permute(0, 2, 1, 3).clone(
+        memory_format=torch.contiguous_format)
+
+
+def _by_rows(tiles: torch.Tensor, n: int) -> torch.Tensor:
+    """The [E, out, n] bytes of _by_tiles' layout."""
+    E, _, out_f, _ = (int(v) for v in tiles.shape)
+    return tiles.permute(0, 2, 1, 3).reshape(E, out_f, -1)[..., :n]
 
 
 def from_bnb_nf4(*, packed: torch.Tensor, absmax: torch.Tensor, nested_absmax: torch.Tensor,

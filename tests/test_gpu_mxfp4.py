@@ -274,12 +274,15 @@ def test_packed_blocks_load_without_requantising():
     m, wq = _module(2, 64, 128)
     p = m.packed_weight("w1")
     n = CompressedGroupedExperts.from_empty(num_experts=2, quant_format="mxfp4")
-    codes, scales = p.data.view(2, 64, 4, 16).clone(), p.scale.clone()
+    q = mxfp4_quantize(torch.from_numpy(wq).float().cuda())
+    codes, scales = q.codes.view(2, 64, 4, 16).clone(), q.scales.clone()
     n.load_packed_mxfp4("w1", codes=codes, scales=scales, shape=(2, 64, 128))
     codes.zero_()
     assert np.array_equal(_np(n._dequantize("w1", dtype=torch.float32)), wq)
     assert n.packed_buffer_names("w1") == ("w1_mxfp4", "w1_mxfp4_scale")
     assert p.nbytes() == 2 * 64 * (64 + 4)
+    assert all(torch.equal(n.packed_weight("w1").data, t.data) and torch.equal(n.packed_weight("w1").scale, t.scale)
+               for t in (p,))
     one = quant.dequantize(p, experts=slice(1, 2), dtype=torch.float32)
     assert np.array_equal(_np(one)[0], wq[1])
 
