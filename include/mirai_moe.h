@@ -732,6 +732,16 @@ int mx_grouped_linear(const void *x, const int64_t *counts, int64_t num_rows, in
                       const mx_weight *w, const mx_lora *lora, void *out, void *workspace,
                       void *stream);
 
+/*
+ * mx_grouped_linear with the rows cut by each expert's inclusive row end, `offsets` [E]
+ * int32 or int64 (offsets_64), as grouped_linear takes them: the plan of their
+ * differences, formed in one launch. host_err (mapped pinned memory, or NULL) receives
+ * the plan's error count.
+ */
+int mx_grouped_linear_offsets(const void *x, const void *offsets, int offsets_64, int64_t num_rows,
+                              int num_experts, const mx_weight *w, const mx_lora *lora, void *out,
+                              void *workspace, int32_t *host_err, void *stream);
+
 /* Bytes of scratch for mx_mxfp4_grouped_linear (0: invalid sizes). */
 size_t mx_mxfp4_grouped_linear_workspace_size(int64_t num_rows, int num_experts,
                                               int64_t in_features);
@@ -777,6 +787,12 @@ int mx_grouped_linear_backward(const void *grad_out, const void *x, const int64_
                                int64_t num_rows, int num_experts, const mx_weight *w,
                                const mx_lora *lora, void *grad_x, float *grad_a, float *grad_b,
                                void *workspace, void *stream);
+
+/* mx_grouped_linear_backward with the rows cut as mx_grouped_linear_offsets cuts them. */
+int mx_grouped_linear_backward_offsets(const void *grad_out, const void *x, const void *offsets,
+                                       int offsets_64, int64_t num_rows, int num_experts,
+                                       const mx_weight *w, const mx_lora *lora, void *grad_x,
+                                       float *grad_a, float *grad_b, void *workspace, void *stream);
 
 /*
  * Backward of mx_moe_forward (adapter training, frozen base): given

@@ -178,6 +178,9 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "mx_nf4_dq_absmax": (c_int, [POINTER(MxNf4Dq), c_int64, c_int64, _P, _P]),
     "mx_int8_quantize": (c_int, [_P, c_int, c_int64, c_int64, _P, _P, _P]),
     "mx_int8_dequantize": (c_int, [_P, _P, c_int64, c_int64, _P, c_int, _P]),
+    "mx_grouped_linear_offsets": (c_int, [_P, _P, c_int, c_int64, c_int, _W, _L, _P, _P, _P, _P]),
+    "mx_grouped_linear_backward_offsets": (
+        c_int, [_P, _P, _P, c_int, c_int64, c_int, _W, _L, _P, _P, _P, _P, _P]),
     "mx_mxfp4_quantize": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, _P, _P]),
     "mx_mxfp4_dequantize": (c_int, [_P, _P, c_int64, c_int64, _P, c_int, _P]),
     "mx_mxfp4_grouped_linear_workspace_size": (c_size_t, [c_int64, c_int, c_int64]),

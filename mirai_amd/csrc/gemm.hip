@@ -3258,11 +3258,25 @@ extern "C" int mx_moe_for_loop(const void *tokens_sorted, const int64_t *counts,
                              MX_ACT_SILU, w1, w3, w2, l1, l3, l2, out, workspace, stream);
 }
 
-extern "C" int mx_grouped_linear(const void *x, const int64_t *counts, int64_t num_rows,
-                                 int num_experts, const mx_weight *w, const mx_lora *lora,
-                                 void *out, void *workspace, void *stream) {
+namespace mx {
+namespace gemm {
+
+// How the rows of a grouped projection are cut: by counts, or by inclusive row ends.
+struct RowCuts {
+  const int64_t *counts;
+  const void *offsets;
+  bool wide;
+  int32_t *host_err;
+};
+
+int plan_rows(const RowCuts &c, int64_t num_rows, int num_experts, void *ws, hipStream_t s) {
+  return c.counts ? plan_from_counts(c.counts, num_rows, num_experts, ws, s)
+                  : plan_from_offsets(c.offsets, c.wide, num_rows, num_experts, ws, s, c.host_err);
+}
+
+int grouped_linear(const char *name, const void *x, const RowCuts &cuts, int64_t num_rows, int num_experts,
+                   const mx_weight *w, const mx_lora *lora, void *out, void *workspace, void *stream) {
   clear_error();
-  const char *name = "mx_grouped_linear";
   int rc = validate_plan_args(name, num_rows, 1, num_experts);
   if (rc) return rc;
   if (!w) {
@@ -3281,7 +3295,7 @@ extern "C" int mx_grouped_linear(const void *x, const int64_t *counts, int64_t n
     return MX_ERR_INVALID;
   }
   if (num_rows == 0) return MX_OK;
-  if (!x || !counts || !out || !workspace) {
+  if (!x || (!cuts.counts && !cuts.offsets) || !out || !workspace) {
     set_error("%s: x, counts, output and workspace must be non-null", name);
     return MX_ERR_INVALID;
   }
@@ -3290,7 +3304,7 @@ extern "C" int mx_grouped_linear(const void *x, const int64_t *counts, int64_t n
   const LayerLayout L = layer_layout(num_rows, num_experts, in_f, out_f, false, 0, lrc);
   char *ws = static_cast<char *>(workspace);
   const PlanView v = plan_view(ws, L.plan);
-  if ((rc = plan_from_counts(counts, num_rows, num_experts, ws, s))) return rc;
+  if ((rc = plan_rows(cuts, num_rows, num_experts, ws, s))) return rc;
   uint16_t *lora_buf = reinterpret_cast<uint16_t *>(ws + L.off_lora);
   const bool lr = has_lora(lora);
   if (lr) {
@@ -3315,9 +3329,6 @@ extern "C" int mx_grouped_linear(const void *x, const int64_t *counts, int64_t n
   p.ldo = out_f;
   return launch_any<EPI_STORE>(w->format, lr, p, L.plan, v, s);
 }
-
-namespace mx {
-namespace gemm {
 
 // Scratch of the grouped-linear backward: plan | p [S, rc] (the forward's
 // low-rank rows, recomputed) | dz [S, rc] | B^T [E, rc, out] | A^T [E, in, rc].
@@ -3356,13 +3367,27 @@ extern "C" size_t mx_grouped_linear_backward_workspace_size(int64_t num_rows, in
                             lora_width(lora_rank)).bytes;
 }
 
-extern "C" int mx_grouped_linear_backward(const void *grad_out, const void *x,
-                                          const int64_t *counts, int64_t num_rows,
-                                          int num_experts, const mx_weight *w,
-                                          const mx_lora *lora, void *grad_x, float *grad_a,
-                                          float *grad_b, void *workspace, void *stream) {
+extern "C" int mx_grouped_linear(const void *x, const int64_t *counts, int64_t num_rows,
+                                 int num_experts, const mx_weight *w, const mx_lora *lora,
+                                 void *out, void *workspace, void *stream) {
+  return grouped_linear("mx_grouped_linear", x, {counts, nullptr, false, nullptr}, num_rows, num_experts, w,
+                        lora, out, workspace, stream);
+}
+
+extern "C" int mx_grouped_linear_offsets(const void *x, const void *offsets, int offsets_64, int64_t num_rows,
+                                         int num_experts, const mx_weight *w, const mx_lora *lora, void *out,
+                                         void *workspace, int32_t *host_err, void *stream) {
+  return grouped_linear("mx_grouped_linear_offsets", x, {nullptr, offsets, offsets_64 != 0, host_err}, num_rows,
+                        num_experts, w, lora, out, workspace, stream);
+}
+
+namespace mx {
+namespace gemm {
+
+int grouped_linear_backward(const char *name, const void *grad_out, const void *x, const RowCuts &cuts,
+                            int64_t num_rows, int num_experts, const mx_weight *w, const mx_lora *lora,
+                            void *grad_x, float *grad_a, float *grad_b, void *workspace, void *stream) {
   clear_error();
-  const char *name = "mx_grouped_linear_backward";
   int rc = validate_plan_args(name, num_rows, 1, num_experts);
   if (rc) return rc;
   if (!w) {
@@ -3389,7 +3414,7 @@ extern "C" int mx_grouped_linear_backward(const void *grad_out, const void *x,
     return zero_lora_grads(name, num_experts, in_f, out_f, lora, nullptr, nullptr, grad_a,
                            grad_b, nullptr, nullptr, nullptr, nullptr, s);
   }
-  if (!grad_out || !x || !counts || !workspace || (!grad_x && !lr)) {
+  if (!grad_out || !x || (!cuts.counts && !cuts.offsets) || !workspace || (!grad_x && !lr)) {
     set_error("%s: gradient, x, counts and workspace must be non-null", name);
     return MX_ERR_INVALID;
   }
@@ -3397,7 +3422,7 @@ extern "C" int mx_grouped_linear_backward(const void *grad_out, const void *x,
   const LinearBackLayout L = linear_back_layout(num_rows, num_experts, in_f, out_f, lrc);
   char *ws = static_cast<char *>(workspace);
   const PlanView v = plan_view(ws, L.plan);
-  if ((rc = plan_from_counts(counts, num_rows, num_experts, ws, s))) return rc;
+  if ((rc = plan_rows(cuts, num_rows, num_experts, ws, s))) return rc;
   const uint16_t *dy = static_cast<const uint16_t *>(grad_out);
   const uint16_t *xr = static_cast<const uint16_t *>(x);
   uint16_t *prow = reinterpret_cast<uint16_t *>(ws + L.off_p);
@@ -3448,6 +3473,27 @@ extern "C" int mx_grouped_linear_backward(const void *grad_out, const void *x,
   ph.add({dy, out_f, nullptr, out_f}, prow, lrc, lora->rank, grad_b, false);
   ph.add({xr, in_f, nullptr, in_f}, dz, lrc, lora->rank, grad_a, true);
   return ph.run(v, num_experts, s);
+}
+
+}  // namespace gemm
+}  // namespace mx
+
+extern "C" int mx_grouped_linear_backward(const void *grad_out, const void *x,
+                                          const int64_t *counts, int64_t num_rows,
+                                          int num_experts, const mx_weight *w,
+                                          const mx_lora *lora, void *grad_x, float *grad_a,
+                                          float *grad_b, void *workspace, void *stream) {
+  return grouped_linear_backward("mx_grouped_linear_backward", grad_out, x, {counts, nullptr, false, nullptr},
+                                 num_rows, num_experts, w, lora, grad_x, grad_a, grad_b, workspace, stream);
+}
+
+extern "C" int mx_grouped_linear_backward_offsets(const void *grad_out, const void *x, const void *offsets,
+                                                  int offsets_64, int64_t num_rows, int num_experts,
+                                                  const mx_weight *w, const mx_lora *lora, void *grad_x,
+                                                  float *grad_a, float *grad_b, void *workspace, void *stream) {
+  return grouped_linear_backward("mx_grouped_linear_backward_offsets", grad_out, x,
+                                 {nullptr, offsets, offsets_64 != 0, nullptr}, num_rows, num_experts, w, lora,
+                                 grad_x, grad_a, grad_b, workspace, stream);
 }
 
 // ------------------------------------------------------------ expert choice

@@ -188,79 +188,81 @@ struct PlanOut {
   int32_t *host_err;
 };
 
-// Inclusive scan over the 256 threads of a workgroup.
-template <class F>
-__device__ __forceinline__ int64_t scan256(int64_t v, int64_t *buf, F op) {
-  const int t = threadIdx.x;
-  buf[t] = v;
-  __syncthreads();
-  for (int d = 1; d < 256; d <<= 1) {
-    const int64_t o = t >= d ? buf[t - d] : buf[t];
-    const bool use = t >= d;
-    __syncthreads();
-    if (use) buf[t] = op(o, buf[t]);
-    __syncthreads();
+// Inclusive sums over the 256 threads of a workgroup; `total` receives the last.
+__device__ __forceinline__ int64_t scan256(int64_t v, int64_t *buf, int64_t &total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t y = __shfl_up(v, off, 64);
+    v += lane >= off ? y : 0;
   }
-  const int64_t r = buf[t];
+  __syncthreads();  // the last use of buf
+  if (lane == 63) buf[wave] = v;
   __syncthreads();
-  return r;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    v += w < wave ? buf[w] : 0;
+    total += buf[w];
+  }
+  return v;
 }
 
-// The tile list of one workgroup: thread t takes the experts [t per, (t + 1) per).
-// An expert's rows run from the largest end before it to its own end, both held
-// within [0, rows].
+// The tile list, by one workgroup: thread t takes the experts [t per, (t + 1) per).
+// Counts are the differences of the row ends: an end below the one before it, or
+// counts that do not add up, are errors, as in the plans of the other projections.
 __device__ void plan_tiles(const PlanOut &P) {
-  __shared__ int64_t buf[256];
+  __shared__ int64_t buf[4];
+  __shared__ int32_t n_err;
+  if (threadIdx.x == 0) n_err = 0;
   const int per = (P.experts + 255) / 256;
   const int e0 = min(static_cast<int>(threadIdx.x) * per, P.experts), e1 = min(e0 + per, P.experts);
-  auto raw = [&](int e) {
-    return P.wide ? static_cast<const int64_t *>(P.offsets)[e]
-                  : static_cast<int64_t>(static_cast<const int32_t *>(P.offsets)[e]);
+  auto end_of = [&](int e) -> int64_t {
+    return P.wide ? static_cast<const int64_t *>(P.offsets)[e] : static_cast<const int32_t *>(P.offsets)[e];
   };
-  auto held = [&](int64_t v) { return min(max(v, int64_t(0)), P.rows); };
-  int64_t top = 0;
-  for (int e = e0; e < e1; ++e) top = max(top, held(raw(e)));
-  const int64_t upto = scan256(top, buf, [](int64_t a, int64_t b) { return max(a, b); });
-  // The largest end before this thread's experts.
-  buf[threadIdx.x] = upto;
-  __syncthreads();
-  const int64_t before = threadIdx.x ? buf[threadIdx.x - 1] : 0;
-  const int64_t last = buf[255];
-  __syncthreads();
-  int64_t start = before, bad = 0;
-  int64_t tiles = 0;  // tall ones in the low half, short ones in the high half
-  auto tall_of = [](int64_t rows) { return (rows + kTall - kShort - 1) / kTall; };
-  auto short_of = [&](int64_t rows) { return int64_t(rows > tall_of(rows) * kTall); };
+  int64_t rows = 0;
+  int32_t bad = 0;
+  auto count_of = [&](int e) -> int64_t {
+    const int64_t c = end_of(e) - (e > 0 ? end_of(e - 1) : 0);
+    return min(max(c, int64_t(0)), P.rows);
+  };
   for (int e = e0; e < e1; ++e) {
-    const int64_t r = raw(e), end = max(start, held(r));
-    bad += r < start || r > P.rows;
-    tiles += tall_of(end - start) + (short_of(end - start) << 32);
-    start = end;
+    const int64_t c = end_of(e) - (e > 0 ? end_of(e - 1) : 0);
+    bad += c < 0 || c > P.rows;
+    rows += count_of(e);
   }
-  auto add = [](int64_t a, int64_t b) { return a + b; };
-  const int64_t tiles_upto = scan256(tiles, buf, add);
-  const int64_t bad_upto = scan256(bad, buf, add);
-  int64_t at = tiles_upto - tiles;
-  start = before;
-  for (int e = e0; e < e1; ++e) {
-    const int64_t end = max(start, held(raw(e)));
-    int64_t n = tall_of(end - start);
-    for (int64_t i = 0; i < n; ++i)
-      P.tall[(at & 0xffffffff) + i] = int4{e, static_cast<int>(start + i * kTall),
-                                           static_cast<int>(min(end - start - i * kTall, int64_t(kTall))), 0};
-    if (short_of(end - start)) {
-      P.rest[at >> 32] = int4{e, static_cast<int>(start + n * kTall),
-                              static_cast<int>(end - start - n * kTall), 0};
+  int64_t all_rows;
+  const int64_t start0 = scan256(rows, buf, all_rows) - rows;
+  if (bad) atomicAdd(&n_err, bad);
+  // Rows beyond P.rows are never touched, even if the ends disagree.
+  auto each = [&](auto f) {
+    int64_t start = start0;
+    for (int e = e0; e < e1; ++e) {
+      const int64_t end = start + count_of(e);
+      const int64_t lo = min(start, P.rows), hi = min(end, P.rows);
+      const int64_t tall = (hi - lo + kTall - kShort - 1) / kTall;
+      f(e, lo, hi, tall, hi - lo > tall * kTall);
+      start = end;
+    }
+  };
+  int64_t tiles = 0, all_tiles;  // tall ones in the low half, short ones in the high half
+  each([&](int, int64_t, int64_t, int64_t tall, bool rest) { tiles += tall + (static_cast<int64_t>(rest) << 32); });
+  int64_t at = scan256(tiles, buf, all_tiles) - tiles;
+  each([&](int e, int64_t lo, int64_t hi, int64_t tall, bool rest) {
+    for (int64_t i = 0; i < tall; ++i)
+      P.tall[(at & 0xffffffff) + i] = int4{e, static_cast<int>(lo + i * kTall),
+                                           static_cast<int>(min(hi - lo - i * kTall, int64_t(kTall))), 0};
+    if (rest) {
+      P.rest[at >> 32] = int4{e, static_cast<int>(lo + tall * kTall), static_cast<int>(hi - lo - tall * kTall), 0};
       at += int64_t(1) << 32;
     }
-    at += n;
-    start = end;
-  }
-  if (threadIdx.x == 255) {
-    const int32_t errors = static_cast<int32_t>(bad_upto + (last != P.rows));
+    at += tall;
+  });
+  if (threadIdx.x == 0) {
+    const int32_t errors = n_err + (all_rows != P.rows);
     P.head[0] = errors;
-    P.head[1] = static_cast<int32_t>(tiles_upto & 0xffffffff);
-    P.head[2] = static_cast<int32_t>(tiles_upto >> 32);
+    P.head[1] = static_cast<int32_t>(all_tiles & 0xffffffff);
+    P.head[2] = static_cast<int32_t>(all_tiles >> 32);
     if (P.host_err) __hip_atomic_store(P.host_err, errors, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
   }
 }

@@ -67,5 +67,9 @@ int build_plan(const int64_t *top_idx, const void *top_scores, int score_dtype,
                int32_t *host_err = nullptr);
 int plan_from_counts(const int64_t *counts, int64_t num_rows, int num_experts, void *workspace,
                      hipStream_t s);
+// The same from inclusive row ends per expert (int32, or int64 with `wide`): the plan of
+// their differences.
+int plan_from_offsets(const void *offsets, bool wide, int64_t num_rows, int num_experts, void *workspace,
+                      hipStream_t s, int32_t *host_err = nullptr);
 
 }  // namespace mx

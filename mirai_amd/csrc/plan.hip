@@ -325,6 +325,81 @@ __device__ __forceinline__ void wg_exclusive_scan(const int32_t (&v)[N], int32_t
   }
 }
 
+// The plan of rows already in order, from each expert's inclusive row end: counts,
+// segments and the four tile lists in one workgroup, thread t taking experts t, t +
+// 1024, ... The counts are the differences of the ends, so a row end below the one
+// before it is an error and an empty expert, as in plan_scan_kernel. Latency is all
+// there is to it: scans are over lanes, the four lists in one. 64 experts: TODO us
+// against 8 to 10 for plan_scan_kernel after four launches that form the counts.
+__global__ __launch_bounds__(1024) void plan_offsets_kernel(const void *offsets, int wide, int E,
+                                                            int64_t n_rows, PlanView v, int32_t *host_err) {
+  __shared__ int64_t wave_rows[16];
+  __shared__ int32_t scan_tmp[64];
+  __shared__ int32_t n_err;
+  const int t = threadIdx.x, lane = t & 63, wid = t >> 6;
+  if (t == 0) n_err = 0;
+  __syncthreads();
+  auto end_of = [&](int e) -> int64_t {
+    return wide ? static_cast<const int64_t *>(offsets)[e] : static_cast<const int32_t *>(offsets)[e];
+  };
+  int64_t carry = 0;
+  int32_t tiles[4] = {0, 0, 0, 0};
+  for (int e0 = 0; e0 < E; e0 += 1024) {
+    const int e = e0 + t;
+    int64_t count = 0;
+    if (e < E) {
+      count = end_of(e) - (e > 0 ? end_of(e - 1) : 0);
+      if (count < 0 || count > n_rows) {
+        atomicAdd(&n_err, 1);
+        count = count < 0 ? 0 : n_rows;
+      }
+    }
+    int64_t upto = count;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t y = __shfl_up(upto, off, 64);
+      upto += lane >= off ? y : 0;
+    }
+    if (lane == 63) wave_rows[wid] = upto;
+    __syncthreads();
+    int64_t before = carry, all = carry;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      const int64_t r = wave_rows[w];
+      before += w < wid ? r : 0;
+      all += r;
+    }
+    carry = all;
+    // Rows beyond num_rows are never touched, even if the ends disagree.
+    const int64_t lo = min(before + upto - count, n_rows), hi = min(before + upto, n_rows);
+    if (e < E) {
+      v.seg[e] = lo;
+      v.seg[E + e] = hi;
+    }
+    const int32_t total = static_cast<int32_t>(hi - lo), start = static_cast<int32_t>(lo);
+    constexpr int M = kPlanTileM;
+    const int32_t full = total / (2 * M), rem = total - full * 2 * M;
+    const int32_t n[4] = {(total + M - 1) / M, full + (rem > 0 ? 1 : 0), full + (rem > M ? 1 : 0),
+                          rem > 0 && rem <= M ? 1 : 0};
+    int32_t at[4], num[4];
+    wg_exclusive_scan<4>(n, at, num, scan_tmp);
+    for (int j = 0; j < n[0]; ++j) v.tiles[tiles[0] + at[0] + j] = make_int2(e, start + j * M);
+    for (int j = 0; j < n[1]; ++j) v.tiles2[tiles[1] + at[1] + j] = make_int2(e, start + j * 2 * M);
+    for (int j = 0; j < n[2]; ++j) v.tiles2m[tiles[2] + at[2] + j] = make_int2(e, start + j * 2 * M);
+    if (n[3]) v.tilesr[tiles[3] + at[3]] = make_int2(e, start + full * 2 * M);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tiles[i] += num[i];
+    __syncthreads();  // wave_rows
+  }
+  if (t == 0) {
+    *v.num_tiles = tiles[0];
+    *v.num_tiles2 = tiles[1];
+    *v.num_tiles2m = tiles[2];
+    *v.num_tilesr = tiles[3];
+    store_errors(n_err + (carry != n_rows ? 1 : 0), v.err, host_err);
+  }
+}
+
 // The plan in one kernel after the block counts, or in one kernel altogether
 // when a single block holds every slot (n_blocks == 1, no counts passed).
 // Latency is all there is to it (a few hundred KB at most), so the scan is not
@@ -656,6 +731,14 @@ int plan_from_counts(const int64_t *counts, int64_t num_rows, int num_experts, v
                      static_cast<int64_t *>(nullptr),
                      static_cast<int64_t *>(nullptr), static_cast<int32_t *>(nullptr));
   return check_launch("mx_plan_from_counts");
+}
+
+int plan_from_offsets(const void *offsets, bool wide, int64_t num_rows, int num_experts, void *workspace,
+                      hipStream_t s, int32_t *host_err) {
+  const PlanView v = plan_view(workspace, plan_layout(num_rows, num_experts));
+  hipLaunchKernelGGL(plan_offsets_kernel, dim3(1), dim3(1024), 0, s, offsets, wide ? 1 : 0, num_experts,
+                     num_rows, v, host_err);
+  return check_launch("plan from row ends");
 }
 
 int validate_plan_args(const char *name, int64_t num_tokens, int top_k, int num_experts) {

@@ -555,19 +555,26 @@ def sorted_experts(module, tokens, counts):
 
 
 def _grouped_inputs(module, key, x, offsets):
-    """(device, counts [E] int64, bf16 rows, packed weight, adapter or None)."""
+    """(device, row ends [E], bf16 rows, packed weight, adapter or None)."""
     device = nat.require_gpu(x)
-    offs = offsets.detach().to(device=device, dtype=torch.int64)
-    if int(offs.numel()) != module.num_experts:
-        raise ValueError("offsets must hold one inclusive row end per expert.")
-    counts = torch.diff(offs, prepend=offs.new_zeros(1)).contiguous()
+    offs = _row_ends(module, offsets, device)
     packed = module.packed_weight(key)
     in_f = int(packed.shape[2])
     if int(x.shape[-1]) != in_f:
         raise ValueError(f"x has {int(x.shape[-1])} features, weight '{key}' expects {in_f}.")
     xb = x.detach().to(torch.bfloat16).contiguous()
     adapter = module.expert_lora[key] if key in module.expert_lora else None
-    return device, counts, xb, packed, adapter
+    return device, offs, xb, packed, adapter
+
+
+def _row_ends(module, offsets, device):
+    """Inclusive row ends per expert as the kernels take them (int32 or int64)."""
+    if int(offsets.numel()) != module.num_experts:
+        raise ValueError("offsets must hold one inclusive row end per expert.")
+    offs = offsets.detach()
+    if offs.dtype not in (torch.int32, torch.int64) or offs.device != device:
+        offs = offs.to(device=device, dtype=torch.int64)
+    return offs.contiguous()
 
 
 def _single_lora(adapter, device):
@@ -578,7 +585,7 @@ def _single_lora(adapter, device):
             [a, b], adapter.padded_rank())
 
 
-def _grouped_linear_forward(module, key, device, counts, xb, packed, adapter):
+def _grouped_linear_forward(module, key, device, offs, xb, packed, adapter):
     S = int(xb.shape[0])
     out_f = int(packed.shape[1])
     lora, keep, rank = _single_lora(adapter, device)
@@ -586,11 +593,17 @@ def _grouped_linear_forward(module, key, device, counts, xb, packed, adapter):
     lib = nat.load_library()
     ws = nat.workspace(lib.mx_moe_workspace_size(S, 1, module.num_experts, int(packed.shape[2]),
                                                  out_f, rank), device)
-    nat.call("mx_grouped_linear", xb.data_ptr(), counts.data_ptr(), S, module.num_experts,
-             packed.descriptor(), lora, out.data_ptr(), ws.data_ptr(), nat.stream(device))
+    slot = nat.open_error_slot() if S > 0 else None
+    try:
+        nat.call("mx_grouped_linear_offsets", xb.data_ptr(), offs.data_ptr(),
+                 int(offs.dtype == torch.int64), S, module.num_experts, packed.descriptor(), lora,
+                 out.data_ptr(), ws.data_ptr(), None if slot is None else slot[1],
+                 nat.stream(device))
+    except BaseException:
+        nat.drop_error_slot(slot, device)
+        raise
     del keep
-    if S > 0:
-        nat.watch_plan_errors(ws, device, "a grouped_linear call")
+    nat.watch_error_slot(slot, device, "a grouped_linear call")
     return out
 
 
@@ -602,15 +615,16 @@ class _GroupedLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, module, key, x, offsets, *lora_params):
-        device, counts, xb, packed, adapter = _grouped_inputs(module, key, x, offsets)
-        out = _grouped_linear_forward(module, key, device, counts, xb, packed, adapter)
+        device, offs, xb, packed, adapter = _grouped_inputs(module, key, x, offsets)
+        out = _grouped_linear_forward(module, key, device, offs, xb, packed, adapter)
         ctx.module, ctx.key, ctx.x_dtype = module, key, x.dtype
-        ctx.save_for_backward(xb, counts)
+        # A copy: the caller may refill its buffer of row ends before the backward.
+        ctx.save_for_backward(xb, offs.clone())
         return out.to(x.dtype)
 
     @staticmethod
     def backward(ctx, grad_out):
-        xb, counts = ctx.saved_tensors
+        xb, offs = ctx.saved_tensors
         module, key = ctx.module, ctx.key
         device = xb.device
         packed = module.packed_weight(key)
@@ -634,9 +648,9 @@ class _GroupedLinear(torch.autograd.Function):
         lib = nat.load_library()
         ws = nat.workspace(lib.mx_grouped_linear_backward_workspace_size(S, E, in_f, out_f, rank),
                            device)
-        nat.call("mx_grouped_linear_backward", g.data_ptr(), xb.data_ptr(), counts.data_ptr(), S,
-                 E, packed.descriptor(), lora, nat.ptr(grad_x), nat.ptr(ga), nat.ptr(gb),
-                 ws.data_ptr(), nat.stream(device))
+        nat.call("mx_grouped_linear_backward_offsets", g.data_ptr(), xb.data_ptr(), offs.data_ptr(),
+                 int(offs.dtype == torch.int64), S, E, packed.descriptor(), lora, nat.ptr(grad_x),
+                 nat.ptr(ga), nat.ptr(gb), ws.data_ptr(), nat.stream(device))
         del keep
         grads = [grad_x.to(ctx.x_dtype) if need_x else None, None]
         if adapter is None:
@@ -660,12 +674,7 @@ def _mxfp4_grouped_forward(module, key, x, offsets):
         raise ValueError(f"x has shape {tuple(x.shape)}, weight '{key}' expects [rows, {in_f}].")
     if not x.is_floating_point():
         raise ValueError(f"x must be floating point, got {x.dtype}.")
-    if int(offsets.numel()) != module.num_experts:
-        raise ValueError("offsets must hold one inclusive row end per expert.")
-    offs = offsets.detach()
-    if offs.dtype not in (torch.int32, torch.int64) or offs.device != device:
-        offs = offs.to(device=device, dtype=torch.int64)
-    offs = offs.contiguous()
+    offs = _row_ends(module, offsets, device)
     rows = x.detach()
     if rows.dtype not in (torch.bfloat16, torch.float32):
         rows = rows.float()
@@ -699,7 +708,8 @@ class _MxGroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, module, key, x, offsets):
         ctx.module, ctx.key, ctx.x_dtype = module, key, x.dtype
-        ctx.save_for_backward(offsets)
+        # A copy: the caller may refill its buffer of row ends before the backward.
+        ctx.save_for_backward(offsets.detach().clone())
         return _mxfp4_grouped_forward(module, key, x, offsets)
 
     @staticmethod
@@ -707,8 +717,7 @@ class _MxGroupedLinear(torch.autograd.Function):
         module, key = ctx.module, ctx.key
         (offsets,) = ctx.saved_tensors
         device = grad_out.device
-        offs = offsets.to(device=device, dtype=torch.int64)
-        counts = torch.diff(offs, prepend=offs.new_zeros(1)).contiguous()
+        offs = _row_ends(module, offsets, device)
         packed = module.packed_weight(key)
         _, out_f, in_f = packed.shape
         g = grad_out.detach().to(torch.bfloat16).contiguous()
@@ -719,9 +728,10 @@ class _MxGroupedLinear(torch.autograd.Function):
                            device)
         # Without adapters the entry point reads no x: any address stands for it.
         with nat.on_device(device):
-            nat.call("mx_grouped_linear_backward", g.data_ptr(), g.data_ptr(), counts.data_ptr(), S,
-                     E, packed.descriptor(), nat.MxLora(None, None, 0, 0.0), grad_x.data_ptr(), None,
-                     None, ws.data_ptr(), nat.stream(device))
+            nat.call("mx_grouped_linear_backward_offsets", g.data_ptr(), g.data_ptr(), offs.data_ptr(),
+                     int(offs.dtype == torch.int64), S, E, packed.descriptor(),
+                     nat.MxLora(None, None, 0, 0.0), grad_x.data_ptr(), None, None, ws.data_ptr(),
+                     nat.stream(device))
         return None, None, grad_x.to(ctx.x_dtype), None
 
 
@@ -741,5 +751,5 @@ def grouped_projection(module, key, x, offsets, activations="bf16"):
     params = [] if adapter is None else [adapter.lora_a, adapter.lora_b]
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *params)):
         return _GroupedLinear.apply(module, key, x, offsets, *params)
-    device, counts, xb, packed, adapter = _grouped_inputs(module, key, x, offsets)
-    return _grouped_linear_forward(module, key, device, counts, xb, packed, adapter).to(x.dtype)
+    device, offs, xb, packed, adapter = _grouped_inputs(module, key, x, offsets)
+    return _grouped_linear_forward(module, key, device, offs, xb, packed, adapter).to(x.dtype)

@@ -207,6 +207,36 @@ def test_grouped_linear_gradient(E, out_f, in_f, ends, activations):
         assert torch.equal(y, m.grouped_linear("w1", x, offsets=offs, activations=activations))
 
 
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+def test_row_ends_may_be_refilled_before_the_backward(activations):
+    m, wq = _module(2, 64, 128)
+    offs = torch.tensor([3, 8], dtype=torch.int32, device="cuda")
+    x = torch.randn(8, 128, device="cuda").bfloat16().requires_grad_(True)
+    dy = torch.randn(8, 64, device="cuda").bfloat16()
+    y = m.grouped_linear("w1", x, offsets=offs, activations=activations)
+    offs.fill_(8)
+    y.backward(dy)
+    dx, mag = _reference(_np(dy).astype(np.float64), wq.transpose(0, 2, 1), [3, 8])
+    assert (np.abs(_np(x.grad).astype(np.float64) - dx) <= _bound(dx, mag, 64, torch.bfloat16)).all()
+
+
+@pytest.mark.parametrize("experts", [1, 3, 255, 256, 257, 1024, 1500])
+def test_row_ends_of_many_experts(experts):
+    g = torch.Generator().manual_seed(experts)
+    counts = torch.randint(0, 4, (experts,), generator=g)
+    counts[::3] = 0
+    counts[0] = 300
+    ends = counts.cumsum(0)
+    m, wq = _module(experts, 64, 64, seed=experts)
+    x = torch.randn(int(ends[-1]), 64, generator=g).bfloat16()
+    for activations in ("bf16", "mxfp4"):
+        got = m.grouped_linear("w1", x.cuda(), offsets=ends.cuda(), activations=activations)
+        xr = x.double().numpy() if activations == "bf16" else omx.roundtrip(x.double().numpy())
+        y, mag = _reference(xr, wq, ends.tolist())
+        assert (np.abs(_np(got).astype(np.float64) - y) <= _bound(y, mag, 64, torch.bfloat16)).all()
+    mirai_amd.check_route_errors()
+
+
 def test_rows_give_the_same_bits_alone_and_together():
     m, _ = _module(2, 256, 512)
     x = torch.randn(700, 512, device="cuda").bfloat16()
@@ -236,9 +266,10 @@ def test_mxfp4_offsets_that_do_not_match_are_reported():
     whole = m.grouped_linear("w1", x, offsets=torch.tensor([2, 5, 8], device="cuda"), activations="mxfp4")
     mirai_amd.check_route_errors()
     for ends in ([2, 5, 7], [2, 1, 8], [2, 5, 9], [-1, 5, 8], [0, 0, 0]):
-        m.grouped_linear("w1", x, offsets=torch.tensor(ends, device="cuda"), activations="mxfp4")
-        with pytest.raises(mirai_amd.RouteIndexError):
-            mirai_amd.check_route_errors()
+        for activations in ("mxfp4", "bf16"):
+            m.grouped_linear("w1", x, offsets=torch.tensor(ends, device="cuda"), activations=activations)
+            with pytest.raises(mirai_amd.RouteIndexError):
+                mirai_amd.check_route_errors()
     again = m.grouped_linear("w1", x, offsets=torch.tensor([2, 5, 8], device="cuda"), activations="mxfp4")
     assert torch.equal(whole, again)
     mirai_amd.check_route_errors()
