@@ -13,13 +13,11 @@ namespace {
 constexpr int kUnroll = 4;  // groups of 8 elements per thread
 
 // Groups of 8 elements in order of (row, group of the row): four consecutive ones
-// are a block and meet in a quad of lanes. Codes and scales lie by row or, TILED, as
-// the product reads them: [ceil(cols / 128)][rows][64] and [ceil(cols / 128)][rows][4],
-// zeros past the row's blocks.
-template <bool BF16, bool TILED>
-__device__ __forceinline__ void quantize_groups(const void *x, int64_t rows, int64_t cols,
-                                                int64_t ldx, bool vec, uint8_t *codes,
-                                                uint8_t *scales, int64_t chunk) {
+// are a block and meet in a quad of lanes.
+template <bool BF16>
+__global__ __launch_bounds__(256) void quantize_kernel(const void *x, int64_t rows, int64_t cols,
+                                                       int64_t ldx, bool vec, uint8_t *codes,
+                                                       uint8_t *scales) {
   const int64_t per_row = 4 * ((cols + kBlock - 1) / kBlock);
   const int64_t total = rows * per_row;
   const bool flat = vec && ldx == cols && cols % kBlock == 0;
@@ -27,7 +25,7 @@ __device__ __forceinline__ void quantize_groups(const void *x, int64_t rows, int
     return total <= 0xffffffffll ? static_cast<uint32_t>(g) / static_cast<uint32_t>(per_row)
                                  : g / per_row;
   };
-  const int64_t g0 = chunk * (256 * kUnroll) + threadIdx.x;
+  const int64_t g0 = static_cast<int64_t>(blockIdx.x) * (256 * kUnroll) + threadIdx.x;
   float v[kUnroll][8];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
@@ -48,38 +46,9 @@ __device__ __forceinline__ void quantize_groups(const void *x, int64_t rows, int
     const int64_t g = g0 + 256 * u;
     if (g >= total) break;
     uint32_t scale;
-    const uint32_t c = quantize8(v[u], scale);
-    if constexpr (!TILED) {
-      reinterpret_cast<uint32_t *>(codes)[g] = c;
-      if ((g & 3) == 0) scales[g >> 2] = static_cast<uint8_t>(scale);
-    } else {
-      const int64_t row = row_of(g), q = g - row * per_row, b = q >> 2;
-      uint32_t *code = reinterpret_cast<uint32_t *>(codes) + ((q >> 4) * rows + row) * 16 + (q & 15);
-      *code = c;
-      uint8_t *at = scales + ((b >> 2) * rows + row) * 4;
-      if (per_row % 16 == 0) {
-        // The 16 lanes of 4 blocks put their scales together.
-        uint32_t w = scale << (8 * (b & 3));
-        w |= __builtin_amdgcn_mov_dpp(static_cast<int>(w), 0x141, 0xf, 0xf, true);  // mirrored half row
-        w |= __builtin_amdgcn_mov_dpp(static_cast<int>(w), 0x140, 0xf, 0xf, true);  // mirrored row
-        if ((g & 15) == 0) *reinterpret_cast<uint32_t *>(at) = w;
-      } else if ((g & 3) == 0) {
-        at[b & 3] = static_cast<uint8_t>(scale);
-        if (b == (per_row >> 2) - 1)
-          for (int i = (b & 3) + 1; i < 4; ++i) at[i] = 0;
-      }
-      // The row's codes past its last group.
-      if (q == per_row - 1)
-        for (int i = 1; i < 16 - static_cast<int>(q & 15); ++i) code[i] = 0;
-    }
+    reinterpret_cast<uint32_t *>(codes)[g] = quantize8(v[u], scale);
+    if ((g & 3) == 0) scales[g >> 2] = static_cast<uint8_t>(scale);
   }
-}
-
-template <bool BF16>
-__global__ __launch_bounds__(256) void quantize_kernel(const void *x, int64_t rows, int64_t cols,
-                                                       int64_t ldx, bool vec, uint8_t *codes,
-                                                       uint8_t *scales) {
-  quantize_groups<BF16, false>(x, rows, cols, ldx, vec, codes, scales, blockIdx.x);
 }
 
 // One group of 8 elements per thread and step.
@@ -267,7 +236,11 @@ __device__ void plan_tiles(const PlanOut &P) {
   }
 }
 
-// The rows' quantisation; the last workgroup forms the tile list meanwhile.
+// The rows' quantisation, codes and scales by 128 columns as the product reads them
+// (zeros past K); the last workgroup forms the tile list meanwhile. A workgroup takes
+// 64 rows of 128 columns: 16 lanes a row, so that reads are runs of 256 bytes (bf16)
+// and a wave's writes of 4 neighbouring rows one run. 131072 x 2048: TODO us; in order
+// of the rows, with codes and scales of a row scattered over the tiles, 155.
 template <bool BF16>
 __global__ __launch_bounds__(256) void rows_kernel(const void *x, int64_t rows, int64_t cols, bool vec,
                                                    uint8_t *codes, uint8_t *scales, PlanOut P) {
@@ -275,9 +248,36 @@ __global__ __launch_bounds__(256) void rows_kernel(const void *x, int64_t rows, 
     plan_tiles(P);
     return;
   }
-  // A run of rows per XCD, so that a line of their scales is written by one L2.
-  const int64_t per = gridDim.x >> 3;
-  quantize_groups<BF16, true>(x, rows, cols, cols, vec, codes, scales, (blockIdx.x & 7) * per + (blockIdx.x >> 3));
+  const int tiles = static_cast<int>((cols + kStep - 1) / kStep);
+  // Runs of workgroups per XCD, the column tiles of the same rows side by side.
+  const int64_t job = static_cast<int64_t>(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const int64_t group = job / tiles, tile = job - group * tiles;
+  const int lane = threadIdx.x & 63, part = lane & 15;
+  const int64_t row0 = group * 64 + 16 * (threadIdx.x >> 6) + (lane >> 4);
+  const int64_t col = tile * kStep + 8 * part;
+  float v[4][8];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t row = row0 + 4 * u;
+    const int n = row < rows && col < cols ? 8 : 0;
+    if (vec && n)
+      load8<BF16>(x, row * cols + col, v[u]);
+    else
+      load8_guarded<BF16>(x, row * cols + col, n, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t row = row0 + 4 * u;
+    uint32_t scale;
+    const uint32_t c = quantize8(v[u], scale);
+    // The 16 lanes of a row's 4 blocks put their scales together.
+    uint32_t w = scale << (8 * (part >> 2));
+    w |= __builtin_amdgcn_mov_dpp(static_cast<int>(w), 0x141, 0xf, 0xf, true);  // mirrored half row
+    w |= __builtin_amdgcn_mov_dpp(static_cast<int>(w), 0x140, 0xf, 0xf, true);  // mirrored row
+    if (row >= rows) continue;
+    reinterpret_cast<uint32_t *>(codes)[(tile * rows + row) * 16 + part] = c;
+    if (part == 0) reinterpret_cast<uint32_t *>(scales)[tile * rows + row] = w;
+  }
 }
 
 struct Product {
@@ -599,7 +599,7 @@ extern "C" int mx_mxfp4_grouped_linear(const void *x, int x_dtype, const void *o
   PlanOut P = {offsets, offsets_64 != 0, num_rows, num_experts, reinterpret_cast<int32_t *>(base),
                reinterpret_cast<int4 *>(base + L.off_tall), reinterpret_cast<int4 *>(base + L.off_short),
                host_err};
-  const int64_t chunks = 8 * ceil_div(ceil_div(num_rows * (K / 8), 256 * kUnroll), 8);
+  const int64_t chunks = 8 * ceil_div(ceil_div(num_rows, 64) * ceil_div(K, kStep), 8);
   const int64_t n_tiles = ceil_div(N, 128);
   const int64_t grid = 8 * (ceil_div(L.max_tall * n_tiles, 8) + ceil_div(L.max_short * n_tiles, 8));
   if (int rc = grid_ok(name, std::max(chunks + 1, grid))) return rc;
