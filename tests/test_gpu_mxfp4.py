@@ -190,6 +190,28 @@ def test_grouped_linear(case, activations, dtype):
         assert (err <= _bound(y, mag, in_f, dtype)).all(), float((err - _bound(y, mag, in_f, dtype)).max())
 
 
+# Rows and columns enough for the 256 x 256 tiles: last tiles of few rows, of few
+# columns, of both; one to five stages of K, odd halves.
+WIDE = [(1, 1720, 64, [20000]), (2, 1624, 192, [9000, 20800]), (4, 1624, 384, [100, 229, 12000, 21000]),
+        (2, 2048, 128, [16513, 16640]), (3, 1544, 576, [0, 22000, 22129]), (1, 1288, 320, [26300])]
+
+
+@pytest.mark.parametrize("case", WIDE, ids=str)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_mxfp4_product_of_many_rows(case, dtype):
+    E, out_f, in_f, ends = case
+    m, wq = _module(E, out_f, in_f, seed=out_f)
+    x = torch.randn(ends[-1], in_f, generator=torch.Generator().manual_seed(3)).to(dtype)
+    y, mag = _reference(omx.roundtrip(x.double().numpy()), wq, ends)
+    offs = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    for _ in range(2):
+        got = m.grouped_linear("w1", x.cuda(), offsets=offs, activations="mxfp4")
+        err = np.abs(_np(got).astype(np.float64) - y)
+        assert (err <= _bound(y, mag, in_f, dtype)).all(), float((err - _bound(y, mag, in_f, dtype)).max())
+    some = m.grouped_linear("w1", x[:300].cuda(), offsets=offs.clamp(max=300), activations="mxfp4")
+    assert torch.equal(some, got[:300])
+
+
 @pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
 @pytest.mark.parametrize("E,out_f,in_f,ends", [(1, 64, 64, [1]), (4, 128, 320, [1, 1, 34, 100]),
                                                (3, 320, 128, [200, 200, 461])])
