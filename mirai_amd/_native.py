@@ -292,6 +292,10 @@ def require_gpu(*tensors: torch.Tensor) -> torch.device:
     """Device of the given tensors; raises unless they share one ROCm GPU."""
     load_library()
     devices = {t.device for t in tensors if t is not None}
+    if len(devices) == 1:
+        (device,) = devices
+        if device.type == "cuda":  # so there is a GPU
+            return device
     if not torch.cuda.is_available():
         raise NativeLibraryError("mirai_amd kernels need a ROCm GPU (torch.cuda is unavailable).")
     if len(devices) != 1:

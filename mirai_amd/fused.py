@@ -557,6 +557,7 @@ def sorted_experts(module, tokens, counts):
 def _grouped_inputs(module, key, x, offsets):
     """(device, row ends [E], bf16 rows, packed weight, adapter or None)."""
     device = nat.require_gpu(x)
+    nat.poll_route_errors()
     offs = _row_ends(module, offsets, device)
     packed = module.packed_weight(key)
     in_f = int(packed.shape[2])

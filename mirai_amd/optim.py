@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import torch
 
 from . import _native as nat
@@ -59,6 +60,11 @@ class _Group:
             total += _blocks(p.numel()) * STATE_BLOCK
         self.total = total
         self.bits = bits
+        # Rows of mx_adamw_tensor: addresses (filled per step), length, place, index.
+        self.table = np.zeros((len(params), 5), dtype=np.int64)
+        self.table[:, 2] = [p.numel() for p in params]
+        self.table[:, 3] = self.at
+        self.table[:, 4] = range(len(params))
 
         def zeros(n, dtype, value=0):
             return torch.full((n,), value, dtype=dtype, device=self.device)
@@ -235,25 +241,27 @@ class AdapterAdamW(torch.optim.Optimizer):
 
     def _step_group(self, gi: int) -> None:
         group = self.param_groups[gi]
-        live = [(i, p) for i, p in enumerate(group["params"]) if p.grad is not None]
-        if not live:
+        params = group["params"]
+        grads = [p.grad for p in params]
+        if all(g is None for g in grads):
             return
         held = self._group(gi)
-        capturing = torch.cuda.is_current_stream_capturing()
-        if capturing and not group["capturable"]:
+        device, host_steps = held.device, held.steps is None
+        if host_steps and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdapterAdamW.step() is captured into a graph only with capturable=True: "
                                "its step counts live on the host otherwise.")
         # One call per (step, type) among the tensors: usually one.
         calls: dict = {}
-        keep, touched = [], []
-        for i, p in live:
-            g = p.grad
-            if p.device != held.device:
-                raise ValueError(f"a parameter moved from {held.device} to {p.device} under its "
-                                 "optimiser.")
-            if g.is_sparse or g.layout != torch.strided:
+        keep, entries, touched = [], [], []
+        strided = torch.strided
+        for i, (p, g) in enumerate(zip(params, grads)):
+            if g is None:
+                continue
+            if p.device != device:
+                raise ValueError(f"a parameter moved from {device} to {p.device} under its optimiser.")
+            if g.layout is not strided:
                 raise ValueError("AdapterAdamW takes dense gradients.")
-            if g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
+            if g.dtype is not p.dtype or g.device != device or g.shape != p.shape:
                 raise ValueError(f"a gradient must have its parameter's shape, type and device, got "
                                  f"{tuple(g.shape)} {g.dtype} {g.device}.")
             if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
@@ -262,32 +270,41 @@ class AdapterAdamW(torch.optim.Optimizer):
             entry = self.state[p]
             if not entry:
                 entry.update(held.views(i, p))
-                entry["step"] = held.steps[i] if held.steps is not None else 0
-            step = 0
-            if held.steps is None:
-                entry["step"] = step = int(entry["step"]) + 1
-            calls.setdefault((step, p.dtype), []).append(
-                (p.data_ptr(), g.data_ptr(), p.numel(), held.at[i], i))
+                entry["step"] = 0 if host_steps else held.steps[i]
+            step = int(entry["step"]) + 1 if host_steps else 0
+            at = calls.setdefault((step, p.dtype), ([], [], []))
+            at[0].append(i)
+            at[1].append(p.data_ptr())
+            at[2].append(g.data_ptr())
+            entries.append((entry, step))
             touched.append(p)
         lr = group["lr"]
         lr_ptr = None
         if isinstance(lr, torch.Tensor):
-            if lr.device != held.device:
-                raise ValueError(f"lr lives on {lr.device}, the parameters on {held.device}.")
+            if lr.device != device:
+                raise ValueError(f"lr lives on {lr.device}, the parameters on {device}.")
             lr_ptr, lr = lr.data_ptr(), 0.0
+        flats = held.flats
         config = nat.MxAdamwConfig(
             lr=float(lr), beta1=group["betas"][0], beta2=group["betas"][1], eps=group["eps"],
             weight_decay=group["weight_decay"], seed=group["seed"], group=gi, state_bits=held.bits,
-            exp_avg=held.flats[0].data_ptr(), exp_avg_sq=held.flats[1].data_ptr(),
-            exp_avg_e=held.flats[2].data_ptr() if held.bits == 8 else None,
-            exp_avg_sq_e=held.flats[3].data_ptr() if held.bits == 8 else None,
+            exp_avg=flats[0].data_ptr(), exp_avg_sq=flats[1].data_ptr(),
+            exp_avg_e=flats[2].data_ptr() if held.bits == 8 else None,
+            exp_avg_sq_e=flats[3].data_ptr() if held.bits == 8 else None,
             steps=nat.ptr(held.steps), scalars=nat.ptr(held.scalars), lr_ptr=lr_ptr)
-        with nat.on_device(held.device):
-            for (step, dtype), rows in calls.items():
+        with nat.on_device(device):
+            for (step, dtype), (index, p_ptrs, g_ptrs) in calls.items():
                 config.step, config.dtype = step, nat.dtype_code(dtype)
-                table = (nat.MxAdamwTensor * len(rows))(*rows)
-                nat.call("mx_adamw_step", table, len(rows), ctypes.byref(config),
-                         nat.stream(held.device))
+                # mx_adamw_tensor rows: five 64-bit fields.
+                table = held.table[index]
+                table[:, 0] = p_ptrs
+                table[:, 1] = g_ptrs
+                nat.call("mx_adamw_step", table.ctypes.data, len(index), ctypes.byref(config),
+                         nat.stream(device))
+        # Counted once the step is queued: a refused one leaves the state as it was.
+        if host_steps:
+            for entry, step in entries:
+                entry["step"] = step
         # The kernel writes through raw pointers: what caches by version has to see it.
         torch.autograd.graph.increment_version(touched)
         del keep
