@@ -66,18 +66,39 @@ class _Group:
         self.table[:, 3] = self.at
         self.table[:, 4] = range(len(params))
 
-        def zeros(n, dtype, value=0):
-            return torch.full((n,), value, dtype=dtype, device=self.device)
+        def empty(n, dtype):
+            return torch.empty((n,), dtype=dtype, device=self.device)
 
         if bits == 32:
-            self.flats = (zeros(total, torch.float32), zeros(total, torch.float32))
+            self.flats = (empty(total, torch.float32), empty(total, torch.float32))
         else:
-            # Codes and exponents of zeros.
-            self.flats = (zeros(total, torch.uint8), zeros(total, torch.uint8),
-                          zeros(total // STATE_BLOCK, torch.uint8, 1),
-                          zeros(total // STATE_BLOCK, torch.uint8, 1))
-        self.steps = zeros(len(params), torch.int64) if capturable else None
-        self.scalars = zeros(32 * len(params), torch.uint8) if capturable else None
+            self.flats = (empty(total, torch.uint8), empty(total, torch.uint8),
+                          empty(total // STATE_BLOCK, torch.uint8),
+                          empty(total // STATE_BLOCK, torch.uint8))
+        self.steps = empty(len(params), torch.int64) if capturable else None
+        self.scalars = empty(32 * len(params), torch.uint8) if capturable else None
+        self.clear()
+
+    def clear(self):
+        """No steps taken: moments of zero (codes 0 under the smallest exponent)."""
+        # What the optimiser's state holds of each parameter; None: not begun.
+        self.entries = [None] * len(self.at)
+        for name, flat in zip(_NAMES[self.bits], self.flats):
+            flat.fill_(1 if name.endswith("_e") else 0)
+        if self.steps is not None:
+            self.steps.zero_()
+
+    def begin(self, i, p, entry):
+        """Parameter i's state without a step taken."""
+        views = self.views(i, p)
+        if self.entries[i] is not None:  # its place holds the moments of an entry taken away
+            for name, view in views.items():
+                view.fill_(1 if name.endswith("_e") else 0)
+            if self.steps is not None:
+                self.steps[i] = 0
+        entry.update(views)
+        entry["step"] = 0 if self.steps is None else self.steps[i]
+        self.entries[i] = entry
 
     def views(self, i, p):
         """The state entries of parameter i."""
@@ -188,7 +209,7 @@ class AdapterAdamW(torch.optim.Optimizer):
             entry["step"] = held.steps[i]
         else:
             entry["step"] = step
-        self.state[p] = entry
+        self.state[p] = held.entries[i] = entry
 
     def load_state_dict(self, state_dict) -> None:
         """The moments are taken as stored (type and layout of this optimiser's)."""
@@ -204,12 +225,20 @@ class AdapterAdamW(torch.optim.Optimizer):
         for group, (capturable, bits) in zip(self.param_groups, keep):
             group["capturable"], group["state_bits"] = capturable, bits
             group.setdefault("seed", self.defaults["seed"])
-        self._groups = {}
+        # The flat buffers stay where they are: a captured step goes on with them.
         for gi, (saved, group) in enumerate(zip(saved_groups, self.param_groups)):
             held = self._group(gi)
+            own = {t.untyped_storage().data_ptr() for t in (*held.flats, held.steps) if t is not None}
+            rows = []
             for i, (key, p) in enumerate(zip(saved["params"], group["params"])):
-                if given.get(key):
-                    self._adopt(held, i, p, given[key])
+                entry = given.get(key)
+                if entry:
+                    rows.append((i, p, {
+                        k: v.clone() if isinstance(v, torch.Tensor)
+                        and v.untyped_storage().data_ptr() in own else v for k, v in entry.items()}))
+            held.clear()
+            for row in rows:
+                self._adopt(held, *row)
 
     def flat_moments(self, group: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
         """fp32 (exp_avg, exp_avg_sq) of a parameter group as flat tensors, each
@@ -264,13 +293,20 @@ class AdapterAdamW(torch.optim.Optimizer):
             if g.dtype is not p.dtype or g.device != device or g.shape != p.shape:
                 raise ValueError(f"a gradient must have its parameter's shape, type and device, got "
                                  f"{tuple(g.shape)} {g.dtype} {g.device}.")
+            if p.numel() != held.table[i, 2] or not (p.is_contiguous() or _dense(p)):
+                raise ValueError("a parameter's storage changed under its optimiser.")
             if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
                 g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
                 keep.append(g)
             entry = self.state[p]
-            if not entry:
-                entry.update(held.views(i, p))
-                entry["step"] = 0 if host_steps else held.steps[i]
+            if entry is not held.entries[i]:  # the first step, or state was changed from outside
+                if held.entries[i] is not None and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the state was replaced: take one step before capturing.")
+                if entry:
+                    self._adopt(held, i, p, entry)
+                    entry = self.state[p]
+                else:
+                    held.begin(i, p, entry)
             step = int(entry["step"]) + 1 if host_steps else 0
             at = calls.setdefault((step, p.dtype), ([], [], []))
             at[0].append(i)

@@ -275,6 +275,94 @@ def test_captured_steps(bits):
             ref.step()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_goes_on_after_a_load(bits):
+    params, twins = _params([(300,), (64, 65)]), _params([(300,), (64, 65)])
+    opt = AdapterAdamW(params, **HYPER, state_bits=bits, capturable=True)
+    ref = AdapterAdamW(twins, **HYPER, state_bits=bits)
+    for p, q in zip(params, twins):
+        q.grad = torch.randn(p.shape, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+        p.grad = q.grad.clone()
+    opt.step()
+    ref.step()
+    saved, kept = copy.deepcopy(opt.state_dict()), [p.detach().clone() for p in params]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    graph.replay()
+    opt.load_state_dict(saved)
+    with torch.no_grad():
+        for p, k in zip(params, kept):
+            p.copy_(k)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        ref.step()
+        for p, q in zip(params, twins):
+            assert torch.equal(p, q)
+    # Its own state: nothing changes.
+    before = [t.clone() for t in opt.flat_moments()]
+    opt.load_state_dict(opt.state_dict())
+    for a, b in zip(before, opt.flat_moments()):
+        assert torch.equal(a, b)
+    assert int(opt.state[params[0]]["step"]) == 3
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_taken_away_or_replaced(bits, capturable):
+    params, twins = _params([(300,), (64, 65)]), _params([(300,), (64, 65)])
+    opt = AdapterAdamW(params, **HYPER, state_bits=bits, capturable=capturable)
+    for s in range(2):
+        _set_grads(params, s)
+        opt.step()
+    saved = {k: copy.deepcopy(dict(v)) for k, v in zip("ab", opt.state.values())}
+    values = [p.detach().clone() for p in params]
+
+    def again():
+        for s in range(2):
+            for ps, o in ((params, opt), (twins, ref)):
+                _set_grads(ps, s)
+                o.step()
+            for p, q in zip(params, twins):
+                assert torch.equal(p, q)
+
+    # Emptied: from the first step again.
+    with torch.no_grad():
+        for p, q in zip(params, twins):
+            q.copy_(p)
+    opt.state.clear()
+    ref = AdapterAdamW(twins, **HYPER, state_bits=bits)
+    again()
+    assert int(opt.state[params[1]]["step"]) == 2
+
+    # Replaced: from what the new entries hold.
+    ref = AdapterAdamW(twins, **HYPER, state_bits=bits)
+    with torch.no_grad():
+        for p, q, v in zip(params, twins, values):
+            p.copy_(v)
+            q.copy_(v)
+    for o, ps in ((opt, params), (ref, twins)):
+        for k, p in zip("ab", ps):
+            o.state[p] = copy.deepcopy(saved[k])
+    again()
+    assert int(opt.state[params[1]]["step"]) == 4 == int(ref.state[twins[1]]["step"])
+
+
+def test_parameters_whose_storage_changed_are_refused():
+    for swap in (lambda p: torch.zeros(100, device="cuda"), lambda p: torch.zeros(300, 2, device="cuda")[:, 0]):
+        params = _params([(300,)])
+        opt = AdapterAdamW(params)
+        _set_grads(params, 0)
+        opt.step()
+        params[0].grad = None
+        params[0].data = swap(params[0])
+        params[0].grad = torch.ones_like(params[0])
+        with pytest.raises(ValueError, match="storage changed|shape"):
+            opt.step()
+
+
 def test_refusals():
     params = _params([(300,)])
     opt = AdapterAdamW(params)
