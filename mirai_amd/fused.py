@@ -563,9 +563,14 @@ def _grouped_inputs(module, key, x, offsets):
     in_f = int(packed.shape[2])
     if int(x.shape[-1]) != in_f:
         raise ValueError(f"x has {int(x.shape[-1])} features, weight '{key}' expects {in_f}.")
-    xb = x.detach().to(torch.bfloat16).contiguous()
+    xb = _aligned(x.detach().to(torch.bfloat16).contiguous())
     adapter = module.expert_lora[key] if key in module.expert_lora else None
     return device, offs, xb, packed, adapter
+
+
+def _aligned(t):
+    """t, or a copy where it begins off the kernels' 16 bytes (a view into a buffer)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _row_ends(module, offsets, device):
@@ -639,7 +644,7 @@ class _GroupedLinear(torch.autograd.Function):
         need_b = adapter is not None and ctx.needs_input_grad[5]
         if not (need_x or need_a or need_b):
             return (None,) * (4 + len(ctx.needs_input_grad[4:]))
-        g = grad_out.detach().to(torch.bfloat16).contiguous()
+        g = _aligned(grad_out.detach().to(torch.bfloat16).contiguous())
         grad_x = torch.empty((S, in_f), dtype=torch.bfloat16, device=device) if need_x else None
         ga = gb = None
         if adapter is not None:
@@ -721,7 +726,7 @@ class _MxGroupedLinear(torch.autograd.Function):
         offs = _row_ends(module, offsets, device)
         packed = module.packed_weight(key)
         _, out_f, in_f = packed.shape
-        g = grad_out.detach().to(torch.bfloat16).contiguous()
+        g = _aligned(grad_out.detach().to(torch.bfloat16).contiguous())
         S, E = int(g.shape[0]), module.num_experts
         grad_x = torch.empty((S, in_f), dtype=torch.bfloat16, device=device)
         lib = nat.load_library()

@@ -41,7 +41,7 @@ class MXFP4Tensor:
 
 def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:
     """x [..., cols] (any floating type; bf16 and fp32 are read as they are, others
-    as fp32) in MXFP4. Rows may lie any distance apart."""
+    as fp32) in MXFP4. Rows may lie any distance apart. Carries no gradient."""
     if x.ndim < 1 or int(x.shape[-1]) < 1:
         raise ValueError(f"mxfp4_quantize takes [..., cols] with cols >= 1, got {tuple(x.shape)}.")
     if not x.is_floating_point():

@@ -334,8 +334,8 @@ def test_packed_blocks_load_without_requantising():
     assert np.array_equal(_np(n._dequantize("w1", dtype=torch.float32)), wq)
     assert n.packed_buffer_names("w1") == ("w1_mxfp4", "w1_mxfp4_scale")
     assert p.nbytes() == 2 * 64 * (64 + 4)
-    assert all(torch.equal(n.packed_weight("w1").data, t.data) and torch.equal(n.packed_weight("w1").scale, t.scale)
-               for t in (p,))
+    assert torch.equal(n.packed_weight("w1").data, p.data)
+    assert torch.equal(n.packed_weight("w1").scale, p.scale)
     one = quant.dequantize(p, experts=slice(1, 2), dtype=torch.float32)
     assert np.array_equal(_np(one)[0], wq[1])
 
@@ -376,7 +376,65 @@ def test_products_on_a_side_stream():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+def test_rows_off_the_alignment(activations):
+    m, _ = _module(2, 64, 128)
+    buf = torch.randn(1 + 40 * 128, device="cuda").bfloat16()
+    x = buf[1:].view(40, 128)
+    offs = torch.tensor([7, 40], device="cuda")
+    want = m.grouped_linear("w1", x.clone(), offsets=offs, activations=activations)
+    assert torch.equal(m.grouped_linear("w1", x, offsets=offs, activations=activations), want)
+    wide = torch.randn(40, 300, device="cuda").bfloat16()[:, 5:133]
+    assert torch.equal(m.grouped_linear("w1", wide, offsets=offs, activations=activations),
+                       m.grouped_linear("w1", wide.clone(), offsets=offs, activations=activations))
+    grad = torch.randn(1 + 40 * 64, device="cuda").bfloat16()[1:].view(40, 64)
+    out = []
+    for dy in (grad, grad.clone()):
+        leaf = x.clone().requires_grad_(True)
+        m.grouped_linear("w1", leaf, offsets=offs, activations=activations).backward(dy)
+        out.append(leaf.grad)
+    assert torch.equal(*out)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bad_weights_spoil_their_column_only(bad):
+    g = torch.Generator().manual_seed(0)
+    w = (torch.randn(2, 128, 256, generator=g) * 0.05).bfloat16()
+    w[1, 17, 100] = bad
+    m = CompressedGroupedExperts.from_empty(num_experts=2, quant_format="mxfp4")
+    m.load_dense_weight("w1", w.cuda())
+    for rows in (3, 150):
+        x = torch.randn(2 * rows, 256, generator=g).bfloat16().cuda()
+        offs = torch.tensor([rows, 2 * rows], device="cuda")
+        for activations in ("bf16", "mxfp4"):
+            y = m.grouped_linear("w1", x, offsets=offs, activations=activations)
+            want = torch.zeros(2 * rows, 128, dtype=torch.bool, device="cuda")
+            want[rows:, 17] = True
+            assert torch.equal(y.isnan(), want), (rows, activations)
+
+
 # ------------------------------------------------------------- routed layer
+def test_other_paths_run_over_mxfp4_experts():
+    """Every path of the module over MXFP4 experts against the same module over their
+    values in bf16 (the same products; other tiles add them in another order)."""
+    from mirai_amd import route_topk
+    w = wl.Workload("mxpaths", 16, 300, 256, 192, 8, 2, 8, 16.0, "mxfp4", torch.bfloat16)
+    dense, lora = wl.dense_weights(w), wl.lora_factors(w)
+    m = build_module(w, dense, lora)
+    values = {k: torch.from_numpy(omx.roundtrip(t.float().numpy())).bfloat16() for k, t in dense.items()}
+    b = build_module(wl.Workload("mxpaths", 16, 300, 256, 192, 8, 2, 8, 16.0, "bf16", torch.bfloat16), values, lora)
+    x = wl.tokens(w).cuda()
+    idx, scores = route_topk(wl.router_logits(w).cuda(), w.top_k)
+    counts = torch.tensor([10, 0, 150, 3, 37, 0, 99, 1], device="cuda")
+    picks = torch.stack([torch.randperm(300, device="cuda")[:40] for _ in range(8)]).unsqueeze(0)
+    weight = torch.rand(1, 8, 40, device="cuda")
+    with torch.no_grad():
+        for f in (lambda e: e.run_direct_routed(x, scores, idx), lambda e: e.run_for_loop(x, counts),
+                  lambda e: e.run_expert_choice_routed(x, weight, picks, tokens_per_sample=300)):
+            assert_layer_close(f(m), f(b))
+    assert torch.equal(m.w1, values["w1"].cuda())
+
+
 @pytest.mark.parametrize("tokens,rank", [(1, 0), (9, 16), (200, 16), (700, 40)])
 def test_routed_layer_and_its_gradients(tokens, rank):
     w = wl.Workload("mxfp4", 14, tokens, 256, 192, 8, 2, max(rank, 8), 16.0, "mxfp4", torch.bfloat16)
