@@ -1954,6 +1954,9 @@ int launch_dual(const Params &p, int64_t max_tall, int64_t max_short, hipStream_
 //   512, 256 experts, at 150 142/161, 256 196/210; at K = 512 and 768 NF4 at 110
 //   62/69 63/72, 200 80/85; at K = 640 the two are equal from 48 with even routes,
 //   and skewed ones stay better streamed up to about 96 (55/64 at 56).
+//   MXFP4, even routes and skewed ones: 2048 x 1408, 64 experts, at 32 rows 30/36
+//   65/59, 64 41/45 67/64, 128 65/68 94/87; 768 x 2048, 128 experts, at 32 30/36
+//   68/55, 48 38/43 74/61, 64 40/46 75/72, 128 68/74 102/90: 48 too.
 // * Otherwise both launches cover up to 128 rows with the same tile, and a
 //   tall tile decodes the weights of 129 or more rows once instead of twice:
 //   training steps from 32 rows per expert on are 0.98 to 1.2 times as fast with

@@ -329,8 +329,9 @@ __device__ __forceinline__ void wg_exclusive_scan(const int32_t (&v)[N], int32_t
 // segments and the four tile lists in one workgroup, thread t taking experts t, t +
 // 1024, ... The counts are the differences of the ends, so a row end below the one
 // before it is an error and an empty expert, as in plan_scan_kernel. Latency is all
-// there is to it: scans are over lanes, the four lists in one. 64 experts: TODO us
-// against 8 to 10 for plan_scan_kernel after four launches that form the counts.
+// there is to it: scans are over lanes, the four lists in one. 64 experts, one launch
+// of 5.4 us (64 rows) to 6.8 (16380 rows), where counts formed by four launches and
+// plan_scan_kernel's 8 to 10 us stood before: the call over 64 rows 46 -> 25 us.
 __global__ __launch_bounds__(1024) void plan_offsets_kernel(const void *offsets, int wide, int E,
                                                             int64_t n_rows, PlanView v, int32_t *host_err) {
   __shared__ int64_t wave_rows[16];

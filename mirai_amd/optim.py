@@ -44,6 +44,16 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _check_lr(lr, capturable) -> None:
+    if not isinstance(lr, torch.Tensor):
+        if not float(lr) >= 0.0:
+            raise ValueError(f"Invalid learning rate: {lr}")
+    elif not capturable:
+        raise ValueError("a tensor lr needs capturable=True.")
+    elif lr.numel() != 1 or lr.dtype != torch.float32 or lr.device.type != "cuda":
+        raise ValueError("a tensor lr must hold one fp32 value on the GPU.")
+
+
 class _Group:
     """The flat moments of one parameter group and where each parameter lies."""
 
@@ -127,13 +137,7 @@ class AdapterAdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
                  state_bits: int = 32, seed: int = 0, capturable: bool = False):
-        if isinstance(lr, torch.Tensor):
-            if not capturable:
-                raise ValueError("a tensor lr needs capturable=True.")
-            if lr.numel() != 1 or lr.dtype != torch.float32 or lr.device.type != "cuda":
-                raise ValueError("a tensor lr must hold one fp32 value on the GPU.")
-        elif not float(lr) >= 0.0:
-            raise ValueError(f"Invalid learning rate: {lr}")
+        _check_lr(lr, capturable)
         if not float(eps) >= 0.0:
             raise ValueError(f"Invalid epsilon value: {eps}")
         for i, beta in enumerate(betas):
@@ -161,6 +165,7 @@ class AdapterAdamW(torch.optim.Optimizer):
         try:
             if group["state_bits"] not in (8, 32):
                 raise ValueError("state_bits must be 8 or 32.")
+            _check_lr(group["lr"], group["capturable"])
             if len({id(p) for p in group["params"]}) != len(group["params"]):
                 raise ValueError("a parameter appears twice in one group.")
             for p in group["params"]:
@@ -220,12 +225,17 @@ class AdapterAdamW(torch.optim.Optimizer):
                 if saved.get("state_bits", group["state_bits"]) != group["state_bits"]:
                     raise ValueError(f"the saved moments have state_bits={saved['state_bits']}, this "
                                      f"optimiser {group['state_bits']}.")
-        keep = [(g["capturable"], g["state_bits"]) for g in self.param_groups]
+        keep = [(g["capturable"], g["state_bits"], g["lr"]) for g in self.param_groups]
         super().load_state_dict({"state": {}, "param_groups": saved_groups})
-        for group, (capturable, bits) in zip(self.param_groups, keep):
+        # The flat buffers and a learning rate on the GPU stay where they are: a captured
+        # step goes on with them.
+        for group, (capturable, bits, lr) in zip(self.param_groups, keep):
             group["capturable"], group["state_bits"] = capturable, bits
             group.setdefault("seed", self.defaults["seed"])
-        # The flat buffers stay where they are: a captured step goes on with them.
+            if isinstance(lr, torch.Tensor):
+                group["lr"] = lr.fill_(float(group["lr"]))
+            elif isinstance(group["lr"], torch.Tensor):
+                group["lr"] = float(group["lr"])
         for gi, (saved, group) in enumerate(zip(saved_groups, self.param_groups)):
             held = self._group(gi)
             own = {t.untyped_storage().data_ptr() for t in (*held.flats, held.steps) if t is not None}
@@ -275,6 +285,9 @@ class AdapterAdamW(torch.optim.Optimizer):
         if all(g is None for g in grads):
             return
         held = self._group(gi)
+        if held.total == 0:  # no parameter holds an element
+            return
+        _check_lr(group["lr"], group["capturable"])
         device, host_steps = held.device, held.steps is None
         if host_steps and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdapterAdamW.step() is captured into a graph only with capturable=True: "

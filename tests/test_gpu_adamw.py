@@ -350,6 +350,41 @@ def test_state_taken_away_or_replaced(bits, capturable):
     assert int(opt.state[params[1]]["step"]) == 4 == int(ref.state[twins[1]]["step"])
 
 
+def test_learning_rates_after_construction():
+    params = _params([(300,)])
+    opt = AdapterAdamW(params)
+    _set_grads(params, 0)
+    before = params[0].detach().clone()
+    for lr in (torch.tensor(1e-3, device="cuda"), -1.0, float("nan")):
+        opt.param_groups[0]["lr"] = lr
+        with pytest.raises(ValueError, match="lr|learning rate"):
+            opt.step()
+        with pytest.raises(ValueError, match="lr|learning rate"):
+            opt.add_param_group({"params": _params([(5,)]), "lr": lr})
+    assert torch.equal(params[0], before) and len(opt.param_groups) == 1
+
+    # Between optimisers with a learning rate on the GPU and ones without: the tensor
+    # stays, its value and the numbers go over.
+    rate = torch.tensor(0.5, device="cuda")
+    a = AdapterAdamW(params, lr=rate, capturable=True)
+    b = AdapterAdamW(params, lr=0.25)
+    saved = copy.deepcopy(a.state_dict())
+    a.load_state_dict(b.state_dict())
+    assert a.param_groups[0]["lr"] is rate and float(rate) == 0.25
+    b.load_state_dict(saved)
+    assert b.param_groups[0]["lr"] == 0.5
+    a.load_state_dict(saved)
+    assert a.param_groups[0]["lr"] is rate and float(rate) == 0.5
+
+
+def test_parameters_without_elements():
+    params = _params([(0,), (3, 0)])
+    opt = AdapterAdamW(params)
+    _set_grads(params, 0)
+    opt.step()
+    assert all(t.numel() == 0 for t in opt.flat_moments())
+
+
 def test_parameters_whose_storage_changed_are_refused():
     for swap in (lambda p: torch.zeros(100, device="cuda"), lambda p: torch.zeros(300, 2, device="cuda")[:, 0]):
         params = _params([(300,)])
