@@ -24,8 +24,8 @@
  *                   (uint8 codes, fp32 nested scales, fp32 offsets, 256-entry
  *                   code table), decoded inside the GEMMs
  *   NF4_DQ_KN       NF4_DQ for a weight stored [E, in, out] (as NF4_F32_KN)
- *   MXFP4 weight    by 128 columns: codes uint8 [E, ceil(in/128), out, 64] (e2m1,
- *                   element 2 i of a row in the low nibble of its byte i) and `scale`
+ *   MXFP4 weight    by blocks of 32 columns: codes uint8 [E, 4 ceil(in/128), out, 16]
+ *                   (e2m1, element 2 i of a block in the low nibble of its byte i) and `scale`
  *                   uint8 [E, ceil(in/128), out, 4] (the biased exponents of the
  *                   powers of two of the row's blocks of 32; 255: NaN), zeros past in
  *   NF4_F32_KN      the same codes and fp32 absmax for a weight stored

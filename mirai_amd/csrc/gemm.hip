@@ -49,14 +49,20 @@ constexpr bool is_nf4(int fmt) {
 }
 // OCP microscaled 4-bit floats: e2m1 codes, element 2 i of a row in the low nibble
 // of byte i, and one power of two (its biased exponent, a byte) per 32 columns.
-// Codes lie as [E][ceil(cols / 128)][rows][64] bytes and scales as [..][rows][4], so
-// that neighbouring rows are neighbours.
+// Codes lie by blocks, as [E][4 ceil(cols / 128)][rows][16] bytes, and scales as
+// [E][ceil(cols / 128)][rows][4], so that lanes that take neighbouring rows take
+// neighbouring bytes (with rows of 64 bytes 16380 rows of 128 experts took 83 us, not 79,
+// and 8191 rows of two MXFP4 operands 40, not 38).
 constexpr bool is_mx4(int fmt) { return fmt == MX_FMT_MXFP4; }
-// The 64 code bytes or (BYTES 4) the 4 scales of column tile `tile` of an expert's row.
-template <int BYTES>
-__device__ __forceinline__ const uint8_t *mx4_row(const void *base, int64_t e, int64_t cols, int64_t rows,
-                                                  int64_t tile, int64_t row) {
-  return static_cast<const uint8_t *>(base) + ((e * ((cols + 127) / 128) + tile) * rows + row) * BYTES;
+// The 16 code bytes of block `block` of an expert's row, and the 4 scales of its
+// column tile `tile`.
+__device__ __forceinline__ const uint8_t *mx4_codes(const void *base, int64_t e, int64_t cols, int64_t rows,
+                                                    int64_t block, int64_t row) {
+  return static_cast<const uint8_t *>(base) + ((e * (4 * ((cols + 127) / 128)) + block) * rows + row) * 16;
+}
+__device__ __forceinline__ const uint8_t *mx4_scales(const void *base, int64_t e, int64_t cols, int64_t rows,
+                                                     int64_t tile, int64_t row) {
+  return static_cast<const uint8_t *>(base) + ((e * ((cols + 127) / 128) + tile) * rows + row) * 4;
 }
 // Formats of two codes per byte.
 constexpr bool is_code4(int fmt) { return is_nf4(fmt) || is_mx4(fmt); }
@@ -537,9 +543,9 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
   if (b_valid) {
     const uint8_t *w = static_cast<const uint8_t *>(pick(p.w, which));
     if (is_code4(FMT)) {
-      b_base = (is_mx4(FMT) ? mx4_row<64>(w, e, row_k, wn_rows, 0, bn) : w + wrow * (row_k / 2)) +
-               bh * (T::B_ELEMS / 2);
-      b_absmax = is_mx4(FMT) ? mx4_row<4>(pick(p.wscale, which), e, row_k, wn_rows, 0, bn)
+      b_base = is_mx4(FMT) ? mx4_codes(w, e, row_k, wn_rows, bh * (T::B_ELEMS / 32), bn)
+                           : w + wrow * (row_k / 2) + bh * (T::B_ELEMS / 2);
+      b_absmax = is_mx4(FMT) ? mx4_scales(pick(p.wscale, which), e, row_k, wn_rows, 0, bn)
                              : static_cast<const uint8_t *>(pick(p.wscale, which)) +
                                    wrow * (row_k / kNf4Block) * absmax_bytes(FMT);
       if (kSplitK && p.k_split < p.K) {
@@ -614,9 +620,9 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
       const int64_t wrow = static_cast<int64_t>(e) * (second ? p.wn[1] : p.wn[0]) + krow;
       if (is_mx4(FMT)) {
         // The lane's 32 columns are one block.
-        const int64_t rows = second ? p.wn[1] : p.wn[0], ct = t_col0 / 128, cb = (t_col0 / 32) & 3;
-        rb.q[0] = *reinterpret_cast<const u32x4 *>(mx4_row<64>(w, e, p.N, rows, ct, krow) + 16 * cb);
-        rb.abs = mx4_row<4>(ws, e, p.N, rows, ct, krow)[cb];
+        const int64_t rows = second ? p.wn[1] : p.wn[0];
+        rb.q[0] = *reinterpret_cast<const u32x4 *>(mx4_codes(w, e, p.N, rows, t_col0 / 32, krow));
+        rb.abs = mx4_scales(ws, e, p.N, rows, t_col0 / 128, krow)[(t_col0 / 32) & 3];
       } else if (is_nf4(FMT)) {
         rb.q[0] = *reinterpret_cast<const u32x4 *>(w + wrow * (p.N / 2) + t_col0 / 2);
         rb.abs = load_absmax<FMT>(ws, wrow * (p.N / kNf4Block) + t_col0 / kNf4Block);
@@ -646,10 +652,10 @@ __device__ __forceinline__ void gemm_tile(Params p, int2 tile, int nt, uint8_t *
         ba = b_absmax1;
         ks = kt - static_cast<int>(p.k_split / BK);
       }
-      const int64_t at = is_mx4(FMT) ? (ks >> 1) * 64 * wn_rows + (ks & 1) * 32
-                                     : static_cast<int64_t>(ks) * kBStageBytes;
+      const int64_t at = static_cast<int64_t>(ks) * (is_mx4(FMT) ? 32 * wn_rows : kBStageBytes);
+      const int64_t piece = is_mx4(FMT) ? 16 * wn_rows : 16;
 #pragma unroll
-      for (int q = 0; q < kBRegs; ++q) rb.q[q] = *reinterpret_cast<const u32x4 *>(bb + at + 16 * q);
+      for (int q = 0; q < kBRegs; ++q) rb.q[q] = *reinterpret_cast<const u32x4 *>(bb + at + piece * q);
       rb.abs = is_mx4(FMT)   ? load_absmax<FMT>(ba, (ks >> 1) * 2 * wn_rows + (ks & 1))
                : is_nf4(FMT) ? load_absmax<FMT>(ba, ks * BK / kNf4Block)
                              : 0u;
@@ -1446,16 +1452,17 @@ __device__ __forceinline__ void stream_tile(const Params &p, int2 tile, int nt, 
   // bf16: a lane's 16-byte pieces lie 32 bytes apart (MFMA step s, half h at
   // 32 s + 16 h); the others take kLaneBytes in a row and exchange halves.
   constexpr int kPiece = FMT == MX_FMT_BF16 ? 32 : 16;
-  const uint8_t *codes = (is_mx4(FMT) ? mx4_row<64>(pick(p.w, which), e, p.K, pick(p.wn, which), 0, n_row)
-                                      : static_cast<const uint8_t *>(pick(p.w, which)) +
-                                            wrow * (p.K * (2 * kLaneBytes) / KS)) +
-                         h * (FMT == MX_FMT_BF16 ? 16 : kLaneBytes);
-  // Bytes between two steps of a row.
-  const int64_t step_bytes = is_mx4(FMT) ? 64 * pick(p.wn, which) : 2 * kLaneBytes;
+  const uint8_t *codes = is_mx4(FMT) ? mx4_codes(pick(p.w, which), e, p.K, pick(p.wn, which), kQ * h, n_row)
+                                     : static_cast<const uint8_t *>(pick(p.w, which)) +
+                                           wrow * (p.K * (2 * kLaneBytes) / KS) +
+                                           h * (FMT == MX_FMT_BF16 ? 16 : kLaneBytes);
+  // Bytes between two steps of a row, and between the pieces of a step.
+  const int64_t step_bytes = is_mx4(FMT) ? 2 * kLaneBytes * pick(p.wn, which) : 2 * kLaneBytes;
+  const int64_t piece_bytes = is_mx4(FMT) ? 16 * pick(p.wn, which) : kPiece;
   const uint8_t *absrow = nullptr;
   float i8_scale = 0.0f;
   if constexpr (is_code4(FMT))
-    absrow = is_mx4(FMT) ? mx4_row<4>(pick(p.wscale, which), e, p.K, pick(p.wn, which), 0, n_row)
+    absrow = is_mx4(FMT) ? mx4_scales(pick(p.wscale, which), e, p.K, pick(p.wn, which), 0, n_row)
                          : static_cast<const uint8_t *>(pick(p.wscale, which)) +
                                wrow * (p.K / kNf4Block) * absmax_bytes(FMT);
   if constexpr (FMT == MX_FMT_INT8)
@@ -1478,7 +1485,7 @@ __device__ __forceinline__ void stream_tile(const Params &p, int2 tile, int nt, 
   auto load_codes = [&](int b, Codes &c) __attribute__((always_inline)) {
 #pragma unroll
     for (int q = 0; q < kQ; ++q)
-      c.q[q] = *reinterpret_cast<const u32x4 *>(codes + static_cast<int64_t>(b) * step_bytes + kPiece * q);
+      c.q[q] = *reinterpret_cast<const u32x4 *>(codes + static_cast<int64_t>(b) * step_bytes + piece_bytes * q);
     c.abs = is_mx4(FMT)   ? load_absmax<FMT>(absrow, b * 2 * pick(p.wn, which) + h)
             : is_nf4(FMT) ? load_absmax<FMT>(absrow, 2 * b + h)
                           : 0u;

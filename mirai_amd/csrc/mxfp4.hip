@@ -285,7 +285,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const void *x, int64_t rows, 
 
 struct Product {
   const uint8_t *xc, *xs;  // [ceil(K/128)][S][64], [ceil(K/128)][S][4]
-  const uint8_t *wc, *ws;  // [E, ceil(K/128), N, 64], [E, ceil(K/128), N, 4]
+  const uint8_t *wc, *ws;  // [E, 4 ceil(K/128), N, 16], [E, ceil(K/128), N, 4]
   int64_t S, K, N;
   const int32_t *head;
   const int4 *tall, *rest;
@@ -326,7 +326,10 @@ __device__ __forceinline__ void lds_dma4(const uint8_t *src, uint8_t *dst) {
 // much as the products. Slower, or not worth their registers: scales read by row (a
 // line per row: 462 us, most of it in the address units), two stages of 256 columns
 // and one workgroup per CU (307), persistent tiles of 256 x 256 by 8 waves (258, and
-// 281 for 8192 cubed, though they bring a quarter less to LDS).
+// 281 for 8192 cubed, though they bring a quarter less to LDS). One kernel whose
+// workgroups quantise 128 rows of up to 2048 columns into 136 KB of LDS and then take
+// all columns of their expert against them reads and writes 0.29 GB less, but its
+// workgroups run in step, one on a CU: 404 for both parts, as before.
 template <bool BF16, int MB>
 __device__ __forceinline__ void product_tile(const Product &p, int4 tile, int64_t n0, uint8_t *s0, uint8_t *s1,
                                              uint8_t *s2) {
@@ -343,20 +346,21 @@ __device__ __forceinline__ void product_tile(const Product &p, int4 tile, int64_
   const int n = static_cast<int>(min(p.N - n0, int64_t(128)));
   const int KT = static_cast<int>((p.K + 127) / 128);
   const uint8_t *xc = p.xc + row0 * 64;
-  const uint8_t *wc = p.wc + (e * KT * p.N + n0) * 64;
-  // 16-byte chunks of a stage's rows lie at chunk ^ (row >> 2 & 3): of 16 consecutive
-  // rows one chunk is in 16 different slots of a 256-byte bank line. Rows past the
-  // tile's repeat its last one: their products are not stored.
+  const uint8_t *wc = p.wc + (static_cast<int64_t>(4 * e) * KT * p.N + n0) * 16;
+  // The weights of a stage lie as in memory, block by block. 16-byte chunks of its rows
+  // lie at chunk ^ (row >> 2 & 3): of 16 consecutive rows one chunk is in 16 different
+  // slots of a 256-byte bank line. Rows past the tile's repeat its last one: their
+  // products are not stored.
   const int chunk = 16 * ((lane & 3) ^ ((lane >> 4) & 3));
   uint32_t xo[XD], wo[WD];
 #pragma unroll
   for (int i = 0; i < XD; ++i) xo[i] = 64 * min(16 * (4 * i + wave) + (lane >> 2), m - 1) + chunk;
 #pragma unroll
-  for (int i = 0; i < WD; ++i) wo[i] = 64 * min(16 * (4 * i + wave) + (lane >> 2), n - 1) + chunk;
+  for (int i = 0; i < WD; ++i) wo[i] = 16 * min(64 * ((4 * i + wave) & 1) + lane, n - 1);
   // Scales: 4 bytes of a stage per row, 64 rows per DMA instruction (where there
   // are fewer rows than waves, two waves bring the same ones).
   const uint8_t *xs = p.xs + row0 * 4;
-  const uint8_t *ws = p.ws + (e * KT * p.N + n0) * 4;
+  const uint8_t *ws = p.ws + (static_cast<int64_t>(e) * KT * p.N + n0) * 4;
   const int xg = wave & (BM / 64 - 1), wg = wave & 1;
   const uint32_t xso = 4 * min(64 * xg + lane, m - 1), wso = 4 * min(64 * wg + lane, n - 1);
   auto load = [&](int k, uint8_t *s) __attribute__((always_inline)) {
@@ -364,7 +368,8 @@ __device__ __forceinline__ void product_tile(const Product &p, int4 tile, int64_
 #pragma unroll
     for (int i = 0; i < XD; ++i) lds_dma16(xc + 64 * k * p.S + xo[i], s + (4 * i + wave) * 1024);
 #pragma unroll
-    for (int i = 0; i < WD; ++i) lds_dma16(wc + 64 * k * p.N + wo[i], s + kW + (4 * i + wave) * 1024);
+    for (int i = 0; i < WD; ++i)
+      lds_dma16(wc + 16 * (4 * k + ((4 * i + wave) >> 1)) * p.N + wo[i], s + kW + (4 * i + wave) * 1024);
     lds_dma4(xs + (4 * k * p.S + xso), s + kXS + 256 * xg);
     lds_dma4(ws + (4 * k * p.N + wso), s + kWS + 256 * wg);
     __builtin_amdgcn_sched_barrier(0);
@@ -378,7 +383,7 @@ __device__ __forceinline__ void product_tile(const Product &p, int4 tile, int64_
       for (int q = 0; q < 16; ++q) acc[mb][nb][q] = 0.0f;
   // Half h of a step's 64 columns: chunk 2 s + h, at the first one's place ^ (s << 5).
   const int place0 = li * 64 + ((h ^ ((li >> 2) & 3)) << 4);
-  const int fx = wm * WM * 64 + place0, fw = kW + wn * WN * 64 + place0;
+  const int fx = wm * WM * 64 + place0, fw = kW + h * 2048 + (wn * WN + li) * 16;
   const int sxo = kXS + 4 * (wm * WM + li), swo = kWS + 4 * (wn * WN + li);
   auto step = [&](int k, const uint8_t *s, uint8_t *refill) __attribute__((always_inline)) {
     // The stage has landed once only the DMA of the one after it is under way, and
@@ -407,7 +412,7 @@ __device__ __forceinline__ void product_tile(const Product &p, int4 tile, int64_
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) w[t][nb] = *reinterpret_cast<const u32x4 *>(s + (fw ^ (t << 5)) + 2048 * nb);
+      for (int nb = 0; nb < NB; ++nb) w[t][nb] = *reinterpret_cast<const u32x4 *>(s + fw + 4096 * t + 512 * nb);
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) x[t][mb] = *reinterpret_cast<const u32x4 *>(s + (fx ^ (t << 5)) + 2048 * mb);
     }

@@ -7,10 +7,10 @@
              ``from_bnb_nf4`` keeps the same codes with an fp32 absmax
              (kernel format MX_FMT_NF4_F32).
 * ``int8`` : int8 [E, out, in] and bf16 per-output-row scale [E, out].
-* ``mxfp4``: OCP microscaled 4-bit floats, by 128 columns so that neighbouring
-             rows are neighbours for the kernels: e2m1 codes uint8
-             [E, ceil(in/128), out, 64] (element 2 i of a row in the low nibble of
-             its byte i) and one power of two per 32 elements, as its biased
+* ``mxfp4``: OCP microscaled 4-bit floats, by blocks of 32 columns so that
+             neighbouring rows are neighbours for the kernels: e2m1 codes uint8
+             [E, 4 ceil(in/128), out, 16] (element 2 i of a block in the low nibble
+             of its byte i) and one power of two per 32 elements, as its biased
              exponent, uint8 [E, ceil(in/128), out, 4]; zeros past in. Quantised
              from the given bf16 or fp32 values (no rounding to bf16 before).
 * ``bf16`` : unquantised bf16 [E, out, in].
@@ -141,7 +141,7 @@ def quantize(source: torch.Tensor, fmt: str) -> PackedWeight:
         return PackedWeight("nf4", codes, absmax, (E, out_f, in_f))
     if fmt == "mxfp4":
         q4 = mxfp4_quantize(w)
-        return PackedWeight("mxfp4", _by_tiles(q4.codes, 64), _by_tiles(q4.scales, 4),
+        return PackedWeight("mxfp4", _by_tiles(q4.codes, 16, 64), _by_tiles(q4.scales, 4, 4),
                             (E, out_f, in_f))
     q = torch.empty((E, out_f, in_f), dtype=torch.int8, device=device)
     scale = torch.empty((E, out_f), dtype=torch.bfloat16, device=device)
@@ -215,15 +215,16 @@ def from_mxfp4_blocks(*, codes: torch.Tensor, scales: torch.Tensor,
             raise ValueError(f"MXFP4 {name} must hold {numel} uint8 values, got {int(t.numel())} "
                              f"{t.dtype}.")
     return PackedWeight(
-        "mxfp4", _by_tiles(codes.detach().reshape(E, out_f, in_f // 2), 64),
-        _by_tiles(scales.detach().to(device).reshape(E, out_f, in_f // MX_BLOCK), 4),
+        "mxfp4", _by_tiles(codes.detach().reshape(E, out_f, in_f // 2), 16, 64),
+        _by_tiles(scales.detach().to(device).reshape(E, out_f, in_f // MX_BLOCK), 4, 4),
         (E, out_f, in_f))
 
 
-def _by_tiles(rows: torch.Tensor, width: int) -> torch.Tensor:
-    """[E, out, n] bytes -> a new [E, ceil(n / width), out, width], zeros past n."""
+def _by_tiles(rows: torch.Tensor, width: int, pad: int) -> torch.Tensor:
+    """[E, out, n] bytes -> a new [E, n' / width, out, width] with n' the next multiple
+    of ``pad``, zeros past n."""
     E, out_f, n = (int(v) for v in rows.shape)
-    tiles = -(-n // width)
+    tiles = -(-n // pad) * pad // width
     padded = torch.nn.functional.pad(rows, (0, width * tiles - n))
     return padded.reshape(E, out_f, tiles, width).permute(0, 2, 1, 3).clone(
         memory_format=torch.contiguous_format)
