@@ -16,6 +16,8 @@ bit.
 from __future__ import annotations
 
 import ctypes
+from itertools import chain, islice
+from operator import is_
 
 import numpy as np
 import torch
@@ -70,9 +72,10 @@ class _Group:
             total += _blocks(p.numel()) * STATE_BLOCK
         self.total = total
         self.bits = bits
+        self.numel = [p.numel() for p in params]
         # Rows of mx_adamw_tensor: addresses (filled per step), length, place, index.
         self.table = np.zeros((len(params), 5), dtype=np.int64)
-        self.table[:, 2] = [p.numel() for p in params]
+        self.table[:, 2] = self.numel
         self.table[:, 3] = self.at
         self.table[:, 4] = range(len(params))
 
@@ -292,41 +295,14 @@ class AdapterAdamW(torch.optim.Optimizer):
         if host_steps and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdapterAdamW.step() is captured into a graph only with capturable=True: "
                                "its step counts live on the host otherwise.")
-        # One call per (step, type) among the tensors: usually one.
-        calls: dict = {}
-        keep, entries, touched = [], [], []
-        strided = torch.strided
-        for i, (p, g) in enumerate(zip(params, grads)):
-            if g is None:
-                continue
-            if p.device != device:
-                raise ValueError(f"a parameter moved from {device} to {p.device} under its optimiser.")
-            if g.layout is not strided:
-                raise ValueError("AdapterAdamW takes dense gradients.")
-            if g.dtype is not p.dtype or g.device != device or g.shape != p.shape:
-                raise ValueError(f"a gradient must have its parameter's shape, type and device, got "
-                                 f"{tuple(g.shape)} {g.dtype} {g.device}.")
-            if p.numel() != held.table[i, 2] or not (p.is_contiguous() or _dense(p)):
-                raise ValueError("a parameter's storage changed under its optimiser.")
-            if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
-                g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
-                keep.append(g)
-            entry = self.state[p]
-            if entry is not held.entries[i]:  # the first step, or state was changed from outside
-                if held.entries[i] is not None and torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("the state was replaced: take one step before capturing.")
-                if entry:
-                    self._adopt(held, i, p, entry)
-                    entry = self.state[p]
-                else:
-                    held.begin(i, p, entry)
-            step = int(entry["step"]) + 1 if host_steps else 0
-            at = calls.setdefault((step, p.dtype), ([], [], []))
-            at[0].append(i)
-            at[1].append(p.data_ptr())
-            at[2].append(g.data_ptr())
-            entries.append((entry, step))
-            touched.append(p)
+        addresses = self._plain_case(gi, held, params, grads)
+        if addresses is not None:
+            entries, touched = held.entries, params
+            step = int(entries[0]["step"]) + 1 if host_steps else 0
+            held.table[:, 0], held.table[:, 1] = addresses
+            calls = [(step, params[0].dtype, held.table)]
+        else:
+            calls, keep, entries, touched = self._any_case(held, params, grads)
         lr = group["lr"]
         lr_ptr = None
         if isinstance(lr, torch.Tensor):
@@ -342,18 +318,84 @@ class AdapterAdamW(torch.optim.Optimizer):
             exp_avg_sq_e=flats[3].data_ptr() if held.bits == 8 else None,
             steps=nat.ptr(held.steps), scalars=nat.ptr(held.scalars), lr_ptr=lr_ptr)
         with nat.on_device(device):
-            for (step, dtype), (index, p_ptrs, g_ptrs) in calls.items():
+            for step, dtype, table in calls:
                 config.step, config.dtype = step, nat.dtype_code(dtype)
-                # mx_adamw_tensor rows: five 64-bit fields.
-                table = held.table[index]
-                table[:, 0] = p_ptrs
-                table[:, 1] = g_ptrs
-                nat.call("mx_adamw_step", table.ctypes.data, len(index), ctypes.byref(config),
+                nat.call("mx_adamw_step", table.ctypes.data, len(table), ctypes.byref(config),
                          nat.stream(device))
         # Counted once the step is queued: a refused one leaves the state as it was.
         if host_steps:
-            for entry, step in entries:
-                entry["step"] = step
+            for entry in entries:
+                entry["step"] += 1
         # The kernel writes through raw pointers: what caches by version has to see it.
         torch.autograd.graph.increment_version(touched)
-        del keep
+        del addresses, calls
+
+    def _plain_case(self, gi, held, params, grads):
+        """Addresses of the parameters and gradients where every parameter has a
+        contiguous gradient of its own length, one type and one step count, and state
+        is as the steps before left it; else None. Everything is looked at anew, in few
+        calls per tensor: a step of 72 small tensors 51 us, of which 20 are fixed, and 111
+        with _any_case for all."""
+        numel, contiguous = torch.Tensor.numel, torch.Tensor.is_contiguous
+        try:
+            if not (list(map(numel, grads)) == held.numel == list(map(numel, params))
+                    and all(map(contiguous, params)) and all(map(contiguous, grads))):
+                return None
+        except (TypeError, RuntimeError):  # no gradient, or a sparse one
+            return None
+        if (set(map(torch.Tensor.get_device, chain(params, grads))) != {held.device.index}
+                or len(set(map(torch.Tensor.dtype.__get__, chain(params, grads)))) != 1):
+            return None
+        first = sum(len(g["params"]) for g in self.param_groups[:gi])
+        last = first + len(params)
+        if (len(self.state) < last or not all(map(is_, islice(self.state, first, last), params))
+                or not all(map(is_, islice(self.state.values(), first, last), held.entries))):
+            return None
+        if held.steps is None and len({entry["step"] for entry in held.entries}) != 1:
+            return None
+        return list(map(torch.Tensor.data_ptr, params)), list(map(torch.Tensor.data_ptr, grads))
+
+    def _any_case(self, held, params, grads):
+        """(step, type, mx_adamw_tensor rows) per (step, type) among the tensors that
+        have gradients, what must outlive the launches, and the entries and parameters
+        stepped."""
+        device, host_steps = held.device, held.steps is None
+        found: dict = {}
+        keep, entries, touched = [], [], []
+        for i, (p, g) in enumerate(zip(params, grads)):
+            if g is None:
+                continue
+            if p.device != device:
+                raise ValueError(f"a parameter moved from {device} to {p.device} under its optimiser.")
+            if g.layout is not torch.strided:
+                raise ValueError("AdapterAdamW takes dense gradients.")
+            if g.dtype is not p.dtype or g.device != device or g.shape != p.shape:
+                raise ValueError(f"a gradient must have its parameter's shape, type and device, got "
+                                 f"{tuple(g.shape)} {g.dtype} {g.device}.")
+            if p.numel() != held.numel[i] or not _dense(p):
+                raise ValueError("a parameter's storage changed under its optimiser.")
+            if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+                g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
+                keep.append(g)
+            entry = self.state[p]
+            if entry is not held.entries[i]:  # the first step, or state was changed from outside
+                if held.entries[i] is not None and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the state was replaced: take one step before capturing.")
+                if entry:
+                    self._adopt(held, i, p, entry)
+                    entry = self.state[p]
+                else:
+                    held.begin(i, p, entry)
+            step = int(entry["step"]) + 1 if host_steps else 0
+            at = found.setdefault((step, p.dtype), ([], [], []))
+            at[0].append(i)
+            at[1].append(p.data_ptr())
+            at[2].append(g.data_ptr())
+            entries.append(entry)
+            touched.append(p)
+        calls = []
+        for (step, dtype), (index, p_ptrs, g_ptrs) in found.items():
+            table = held.table[index]
+            table[:, 0], table[:, 1] = p_ptrs, g_ptrs
+            calls.append((step, dtype, table))
+        return calls, keep, entries, touched
