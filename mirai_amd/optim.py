@@ -228,8 +228,14 @@ class AdapterAdamW(torch.optim.Optimizer):
                 if saved.get("state_bits", group["state_bits"]) != group["state_bits"]:
                     raise ValueError(f"the saved moments have state_bits={saved['state_bits']}, this "
                                      f"optimiser {group['state_bits']}.")
+                for what in ("amsgrad", "maximize"):
+                    if saved.get(what):
+                        raise ValueError(f"the saved state is of a run with {what}, which AdapterAdamW "
+                                         "does not offer.")
         keep = [(g["capturable"], g["state_bits"], g["lr"]) for g in self.param_groups]
+        groups = self._groups
         super().load_state_dict({"state": {}, "param_groups": saved_groups})
+        self._groups = groups
         # The flat buffers and a learning rate on the GPU stay where they are: a captured
         # step goes on with them.
         for group, (capturable, bits, lr) in zip(self.param_groups, keep):

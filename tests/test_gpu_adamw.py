@@ -291,7 +291,9 @@ def test_a_captured_step_goes_on_after_a_load(bits):
         opt.step()
     graph.replay()
     graph.replay()
+    held = opt._groups[0]
     opt.load_state_dict(saved)
+    assert opt._groups[0] is held
     with torch.no_grad():
         for p, k in zip(params, kept):
             p.copy_(k)
@@ -375,6 +377,36 @@ def test_learning_rates_after_construction():
     assert b.param_groups[0]["lr"] == 0.5
     a.load_state_dict(saved)
     assert a.param_groups[0]["lr"] is rate and float(rate) == 0.5
+
+
+def test_state_of_the_plain_optimiser():
+    """torch.optim.AdamW's state goes on here: the same formula, a few roundings of
+    fp32 apart (at most 8 per step and value: the update is lr long, the parameter's own
+    roundings 2 more)."""
+    params, twins = _params([(300,), (64, 65)]), _params([(300,), (64, 65)])
+    ref = torch.optim.AdamW(twins, lr=1e-3, weight_decay=0.1)
+    for s in range(3):
+        _set_grads(twins, s)
+        ref.step()
+    opt = AdapterAdamW(params)
+    opt.load_state_dict(copy.deepcopy(ref.state_dict()))
+    with torch.no_grad():
+        for p, q in zip(params, twins):
+            p.copy_(q)
+    assert opt.param_groups[0]["weight_decay"] == 0.1
+    for s in range(3, 5):
+        _set_grads(params, s)
+        _set_grads(twins, s)
+        opt.step()
+        ref.step()
+    eps = torch.finfo(torch.float32).eps / 2
+    for p, q in zip(params, twins):
+        # |m| / sqrt(v) is at most (1 - b1) / sqrt(1 - b2) / (1 - b1 / sqrt(b2)) < 33.
+        assert float((p - q).abs().max()) <= 2 * (8 * eps * 33e-3 + 4 * eps * float(q.abs().max()))
+    assert int(opt.state[params[0]]["step"]) == 5
+    for other in (torch.optim.AdamW(twins, amsgrad=True), torch.optim.AdamW(twins, maximize=True)):
+        with pytest.raises(ValueError, match="amsgrad|maximize"):
+            opt.load_state_dict(other.state_dict())
 
 
 def test_parameters_without_elements():
