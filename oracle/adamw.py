@@ -18,13 +18,16 @@ def mix(x: np.ndarray) -> np.ndarray:
 
 
 def noise(n: int, seed: int, step: int, group: int, at: int = 0):
-    """(m's, v's) 16 random bits of positions at .. at + n - 1 (below 2^32)."""
+    """(m's, v's) 16 random bits of positions at .. at + n - 1."""
+    pos = at + np.arange(n, dtype=np.int64)
+    high = (pos >> 32).astype(np.uint32)
     u = np.uint32
     with np.errstate(over="ignore"):
         key = mix(mix(u(seed)) + u(step))
         if group:
             key = mix(key + u(group))
-        h = mix(np.arange(at, at + n, dtype=np.uint32) + key)
+        key = np.where(high != 0, mix(key + high), key)
+        h = mix((pos & 0xFFFFFFFF).astype(np.uint32) + key)
     return h & u(0xFFFF), h >> u(16)
 
 

@@ -409,6 +409,35 @@ def test_state_of_the_plain_optimiser():
             opt.load_state_dict(other.state_dict())
 
 
+def test_positions_past_32_bits():
+    """8-bit moments behind (and within) a parameter of more than 2^32 elements."""
+    big = torch.nn.Parameter(torch.zeros(2 ** 32 + 77, dtype=torch.bfloat16, device="cuda"))
+    (small,) = _params([(4097,)], torch.bfloat16)
+    opt = AdapterAdamW([big, small], **HYPER, state_bits=8, seed=5)
+    big.grad = torch.zeros_like(big)
+    big.grad[-1] = 3.0
+    _set_grads([small], 2)
+    tail = torch.zeros(77 + 128, dtype=torch.float32, device="cuda")
+    tail[-1] = 3.0
+    opt.step()
+    b1, b2 = HYPER["betas"]
+    for p, g, n, at in ((big, tail, 205, 2 ** 32 - 128), (small, small.grad, 4097, 2 ** 32 + 128)):
+        zero = np.zeros(n, dtype=np.float32)
+        m, v = oadam.averages(g.float().cpu().numpy(), zero, zero, b1, b2)
+        low, high = oadam.noise(n, 5, 1, 0, at)
+        for name, x, noise, ebits, signed in (("exp_avg", m, low, 4, True), ("exp_avg_sq", v, high, 5, False)):
+            codes, exps = oadam.encode(x, ebits, signed, noise)
+            entry = opt.state[p]
+            assert np.array_equal(entry[name + "_q"][-n:].cpu().numpy(), codes)
+            assert np.array_equal(entry[name + "_e"][-exps.size:].cpu().numpy(), exps)
+    assert not opt.state[big]["exp_avg_q"][:-1].any() and not big.detach()[:-1].any() and float(big.detach()[-1]) < 0
+    for flat, entry in zip(opt.flat_moments(), ("exp_avg", "exp_avg_sq")):
+        q, e = opt.state[small][entry + "_q"].cpu().numpy(), opt.state[small][entry + "_e"].cpu().numpy()
+        want = oadam.decode(q, e, 4 if entry == "exp_avg" else 5, entry == "exp_avg")
+        at = 2 ** 32 + 128
+        assert np.array_equal(flat[at:at + 4097].double().cpu().numpy(), want)
+
+
 def test_parameters_without_elements():
     params = _params([(0,), (3, 0)])
     opt = AdapterAdamW(params)

@@ -413,6 +413,58 @@ def test_bad_weights_spoil_their_column_only(bad):
             assert torch.equal(y.isnan(), want), (rows, activations)
 
 
+def test_more_than_32_bits_of_elements():
+    rows, cols = 2 ** 21 + 300, 2112
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    ends = x[:5], x[-300:]
+    for t in ends:
+        t.normal_()
+    q = mxfp4_quantize(x)
+    back = mxfp4_dequantize(q)
+    for t, c, s, v in ((x[:5], q.codes[:5], q.scales[:5], back[:5]),
+                       (x[-300:], q.codes[-300:], q.scales[-300:], back[-300:])):
+        part = mxfp4_quantize(t.clone())
+        assert torch.equal(part.codes, c) and torch.equal(part.scales, s)
+        assert torch.equal(mxfp4_dequantize(part), v)
+    assert not q.codes[5:-300].any() and not back[5:-300].any()
+    del q, back
+    m, _ = _module(2, 64, cols)
+    y = m.grouped_linear("w1", x, offsets=torch.tensor([3, rows], device="cuda"), activations="mxfp4")
+    assert torch.equal(y[-300:], m.grouped_linear("w1", x[-300:].clone(), offsets=torch.tensor([0, 300], device="cuda"),
+                                                  activations="mxfp4"))
+    assert torch.equal(y[:5], m.grouped_linear("w1", x[:5].clone(), offsets=torch.tensor([3, 5], device="cuda"),
+                                               activations="mxfp4"))
+    assert not y[5:-300].any()
+
+
+def test_weights_past_32_bits_of_bytes():
+    E, out_f, in_f = 520, 4096, 4160
+    w = torch.zeros(E, out_f, in_f, dtype=torch.bfloat16, device="cuda")
+    w[-1].normal_(std=0.05)
+    m = CompressedGroupedExperts.from_empty(num_experts=E, quant_format="mxfp4")
+    m.load_dense_weight("w1", w)
+    one = CompressedGroupedExperts.from_empty(num_experts=1, quant_format="mxfp4")
+    one.load_dense_weight("w1", w[-1:].clone())
+    del w
+    assert m.packed_weight("w1").data.numel() > 2 ** 32
+    for rows in (3, 300):
+        x = torch.randn(rows, in_f, device="cuda").bfloat16()
+        dy = torch.randn(rows, out_f, device="cuda").bfloat16()
+        for activations in ("bf16", "mxfp4"):
+            got = []
+            for module, zeros in ((m, E - 1), (one, 0)):
+                leaf = x.clone().requires_grad_(True)
+                offs = torch.tensor([0] * zeros + [rows], device="cuda")
+                y = module.grouped_linear("w1", leaf, offsets=offs, activations=activations)
+                y.backward(dy)
+                got.append((y.detach().float(), leaf.grad.float()))
+            # Other launches may add in another order: fp32 sums and one bf16 rounding a
+            # side, 2^-8 of the value each, and as much again for the sums.
+            for a, b in zip(*got):
+                assert float((a - b).abs().max()) <= 2 ** -6 * float(b.abs().max())
+                assert float(b.abs().max()) > 0.5
+
+
 # ------------------------------------------------------------- routed layer
 def test_other_paths_run_over_mxfp4_experts():
     """Every path of the module over MXFP4 experts against the same module over their
