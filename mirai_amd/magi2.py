@@ -153,7 +153,7 @@ class Magi2GroupedExperts(nn.Module):
 
     ``load_dense_weight`` takes the reference layer's [G, in, out] tensors
     (W_gate, W_up [G, d_head, d_expert]; W_down [G, d_expert, d_head]) and
-    stores them in ``quant_format`` ("nf4", "int8" or "bf16").
+    stores them in ``quant_format`` ("nf4", "int8", "mxfp4" or "bf16").
     """
 
     def __init__(self, *, num_heads: int, num_experts: int, quant_format: str = "nf4",

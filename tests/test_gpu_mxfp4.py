@@ -487,6 +487,68 @@ def test_other_paths_run_over_mxfp4_experts():
     assert torch.equal(m.w1, values["w1"].cuda())
 
 
+def _grad_close(got, want):
+    """The backward's bound against another order of sums: mean 5e-3, 3e-2 of the largest."""
+    got, want = got.detach().float(), want.detach().float()
+    diff = (got - want).abs()
+    assert float(diff.sum()) <= 5e-3 * float(want.abs().sum())
+    assert float(diff.max()) <= 3e-2 * float(want.abs().max())
+
+
+def test_heads_of_experts_over_mxfp4():
+    """MAGI-2's groups, forward and backward, against the same values in bf16."""
+    from mirai_amd import Magi2GroupedExperts
+    H, E, d, f, S = 2, 4, 128, 192, 70
+    g = torch.Generator().manual_seed(2)
+    shapes = {"W_gate": (H * E, d, f), "W_up": (H * E, d, f), "W_down": (H * E, f, d)}
+    dense = {k: (torch.randn(s, generator=g) * 0.08).bfloat16() for k, s in shapes.items()}
+    values = {k: torch.from_numpy(omx.roundtrip(t.transpose(1, 2).float().numpy())).bfloat16().transpose(1, 2)
+              .contiguous() for k, t in dense.items()}
+    probs = torch.rand(H, S, 2, generator=g).cuda()
+    idx = torch.stack([torch.randperm(E, generator=g)[:2] for _ in range(H * S)]).view(H, S, 2).cuda()
+    x = torch.randn(S, H, d, generator=g).bfloat16().cuda()
+    dy = torch.randn(S, H, d, generator=g).bfloat16().cuda()
+    got = []
+    for fmt, w in (("mxfp4", dense), ("bf16", values)):
+        m = Magi2GroupedExperts.from_dense(*(w[k].cuda() for k in shapes), num_heads=H, quant_format=fmt)
+        leaf = x.clone().requires_grad_(True)
+        y = m.execute(leaf, probs, idx)
+        y.backward(dy)
+        got.append((y, leaf.grad))
+    assert_layer_close(got[0][0].detach(), got[1][0].detach())
+    _grad_close(got[0][1], got[1][1])
+
+
+def test_chunks_and_expert_choice_train_over_mxfp4():
+    from mirai_amd import MoETokenChunkPolicy, fused_chunk_runner, route_topk
+    w = wl.Workload("mxchunk", 17, 300, 256, 192, 8, 2, 8, 16.0, "mxfp4", torch.bfloat16)
+    dense, lora = wl.dense_weights(w), wl.lora_factors(w)
+    values = {k: torch.from_numpy(omx.roundtrip(t.float().numpy())).bfloat16() for k, t in dense.items()}
+    m = build_module(w, dense, lora)
+    b = build_module(wl.Workload("mxchunk", 17, 300, 256, 192, 8, 2, 8, 16.0, "bf16", torch.bfloat16), values, lora)
+    x, dy = wl.tokens(w).cuda(), wl.upstream_grad(w).cuda()
+    idx, scores = route_topk(wl.router_logits(w).cuda(), w.top_k)
+    picks = torch.stack([torch.randperm(300, device="cuda")[:40] for _ in range(8)]).unsqueeze(0)
+    weight = torch.rand(1, 8, 40, device="cuda")
+    policy = MoETokenChunkPolicy(token_chunk_size=128)
+
+    def step(e, f):
+        leaf = x.clone().requires_grad_(True)
+        for ad in e.expert_lora.values():
+            ad.lora_a.grad = ad.lora_b.grad = None
+        y = f(e, leaf)
+        y.backward(dy)
+        return [y.detach(), leaf.grad, *(p.grad.clone() for p in e.expert_lora.parameters())]
+
+    for f in (lambda e, t: e.run_direct_routed(t, scores, idx),
+              lambda e, t: policy.execute(t, scores, idx, runner=fused_chunk_runner(e), training=True),
+              lambda e, t: e.run_expert_choice_routed(t, weight, picks, tokens_per_sample=300)):
+        got, want = step(m, f), step(b, f)
+        assert_layer_close(got[0], want[0])
+        for a, c in zip(got[1:], want[1:]):
+            _grad_close(a, c)
+
+
 @pytest.mark.parametrize("tokens,rank", [(1, 0), (9, 16), (200, 16), (700, 40)])
 def test_routed_layer_and_its_gradients(tokens, rank):
     w = wl.Workload("mxfp4", 14, tokens, 256, 192, 8, 2, max(rank, 8), 16.0, "mxfp4", torch.bfloat16)
