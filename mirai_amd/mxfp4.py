@@ -11,6 +11,7 @@ Expert weights take this form with ``quant_format="mxfp4"``, the rows of
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -42,28 +43,29 @@ class MXFP4Tensor:
 def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:
     """x [..., cols] (any floating type; bf16 and fp32 are read as they are, others
     as fp32) in MXFP4. Rows may lie any distance apart. Carries no gradient."""
-    if x.ndim < 1 or int(x.shape[-1]) < 1:
-        raise ValueError(f"mxfp4_quantize takes [..., cols] with cols >= 1, got {tuple(x.shape)}.")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"mxfp4_quantize takes [..., cols] with cols >= 1, got {tuple(shape)}.")
     if not x.is_floating_point():
         raise ValueError(f"mxfp4_quantize takes a floating-point tensor, got {x.dtype}.")
     device = nat.require_gpu(x)
-    x = x.detach()
     if x.dtype not in (torch.bfloat16, torch.float32):
-        x = x.float()
-    cols = int(x.shape[-1])
-    lead = tuple(int(v) for v in x.shape[:-1])
-    # A view where the rows are evenly spaced, else a copy.
-    flat = x.reshape(-1, cols) if x.numel() else x.new_empty((0, cols))
-    if int(flat.stride(1)) != 1 or int(flat.stride(0)) < cols:
-        flat = flat.contiguous()
-    rows = int(flat.shape[0])
+        x = x.detach().float()
+    *lead, cols = shape
+    if x.is_contiguous():
+        flat, rows, ldx = x, math.prod(lead), cols
+    else:
+        # A view where the rows are evenly spaced, else a copy.
+        flat = x.detach().reshape(-1, cols)
+        if flat.stride(1) != 1 or flat.stride(0) < cols:
+            flat = flat.contiguous()
+        rows, ldx = flat.shape[0], max(flat.stride(0), cols)
     blocks = -(-cols // MX_BLOCK)
     codes = torch.empty((*lead, 16 * blocks), dtype=torch.uint8, device=device)
     scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=device)
     with nat.on_device(device):
-        nat.call("mx_mxfp4_quantize", flat.data_ptr(), nat.dtype_code(flat.dtype), rows, cols,
-                 max(int(flat.stride(0)), cols), codes.data_ptr(), scales.data_ptr(),
-                 nat.stream(device))
+        nat.call("mx_mxfp4_quantize", flat.data_ptr(), nat.dtype_code(flat.dtype), rows, cols, ldx,
+                 codes.data_ptr(), scales.data_ptr(), nat.stream(device))
     return MXFP4Tensor(codes, scales, cols)
 
 
@@ -71,10 +73,9 @@ def mxfp4_dequantize(q: MXFP4Tensor, *, dtype: torch.dtype = torch.bfloat16) -> 
     """The [..., cols] values ``q`` stands for, in bf16 or fp32 (both hold them
     exactly, but for scales above 2^125, which only other quantisers produce)."""
     cols, blocks = int(q.cols), -(-int(q.cols) // MX_BLOCK)
-    lead = tuple(int(v) for v in q.codes.shape[:-1])
+    lead = q.codes.shape[:-1]
     if (cols < 1 or q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8
-            or tuple(q.codes.shape) != (*lead, 16 * blocks)
-            or tuple(q.scales.shape) != (*lead, blocks)):
+            or q.codes.shape != (*lead, 16 * blocks) or q.scales.shape != (*lead, blocks)):
         raise ValueError(f"an MXFP4 tensor of {cols} columns holds uint8 codes [..., {16 * blocks}] "
                          f"and scales [..., {blocks}], got {tuple(q.codes.shape)} "
                          f"{q.codes.dtype} and {tuple(q.scales.shape)} {q.scales.dtype}.")
@@ -84,7 +85,7 @@ def mxfp4_dequantize(q: MXFP4Tensor, *, dtype: torch.dtype = torch.bfloat16) -> 
     if codes.data_ptr() % 4:
         codes = codes.clone()
     out = torch.empty((*lead, cols), dtype=dtype, device=device)
-    rows = codes.numel() // (16 * blocks)
+    rows = math.prod(lead)
     with nat.on_device(device):
         nat.call("mx_mxfp4_dequantize", codes.data_ptr(), scales.data_ptr(), rows, cols,
                  out.data_ptr(), code, nat.stream(device))
