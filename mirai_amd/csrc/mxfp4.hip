@@ -600,8 +600,9 @@ extern "C" int mx_mxfp4_grouped_linear(const void *x, int x_dtype, const void *o
     set_error("%s: x, offsets, output and workspace must be non-null", name);
     return MX_ERR_INVALID;
   }
-  if (!aligned16(w->data) || !aligned16(out) || !aligned16(workspace)) {
-    set_error("%s: weight codes, output and workspace must be 16-byte aligned", name);
+  if (!aligned16(w->data) || !aligned16(out) || !aligned16(workspace) ||
+      reinterpret_cast<uintptr_t>(w->scale) % 4 != 0) {
+    set_error("%s: weight codes, output and workspace must be 16-byte and weight scales 4-byte aligned", name);
     return MX_ERR_INVALID;
   }
   hipStream_t s = as_stream(stream);

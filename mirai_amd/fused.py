@@ -713,6 +713,9 @@ class _MxGroupedLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, module, key, x, offsets):
+        out_f = int(module.packed_weight(key).shape[1])
+        if out_f % 64:
+            raise ValueError(f"the gradient of x needs out_features a multiple of 64, got {out_f}.")
         ctx.module, ctx.key, ctx.x_dtype = module, key, x.dtype
         # A copy: the caller may refill its buffer of row ends before the backward.
         ctx.save_for_backward(offsets.detach().clone())

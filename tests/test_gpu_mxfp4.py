@@ -307,6 +307,9 @@ def test_mxfp4_refusals_on_the_gpu():
         m.grouped_linear("w1", x, offsets=offs[:1], activations="mxfp4")
     with pytest.raises(ValueError, match="floating"):
         m.grouped_linear("w1", x.int(), offsets=offs, activations="mxfp4")
+    odd, _ = _module(2, 72, 64)
+    with pytest.raises(ValueError, match="multiple of 64"):
+        odd.grouped_linear("w1", x.clone().requires_grad_(True), offsets=offs, activations="mxfp4")
     m.attach_expert_lora(tensor_name="w1", adapter_name="t", rank=8, alpha=8.0)
     with pytest.raises(ValueError, match="adapter"):
         m.grouped_linear("w1", x, offsets=offs, activations="mxfp4")

@@ -55,6 +55,7 @@ def test_grouped_linear_refuses():
                   (nat.MxWeight(nat.FMT_MXFP4, 16, 16, 128, 96), {}),
                   (nat.MxWeight(nat.FMT_MXFP4, 16, 16, 12, 64), {}),
                   (nat.MxWeight(nat.FMT_MXFP4, 8, 16, 128, 64), {}),
+                  (nat.MxWeight(nat.FMT_MXFP4, 16, 18, 128, 64), {}),
                   (good, {"rows": -1}), (good, {"rows": 1 << 31}), (good, {"E": 0}), (good, {"E": 9000}),
                   (good, {"dt": 3}), (good, {"odt": 3}), (good, {"x": None}), (good, {"offs": None}),
                   (good, {"out": None}), (good, {"out": 8}), (good, {"ws": None}), (good, {"ws": 8})):
