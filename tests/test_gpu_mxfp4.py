@@ -399,6 +399,23 @@ def test_rows_off_the_alignment(activations):
     assert torch.equal(*out)
 
 
+@pytest.mark.parametrize("in_f", [64, 320, 384])
+@pytest.mark.parametrize("rows", [2, 40, 300])
+def test_infinite_rows_give_what_their_products_do(in_f, rows):
+    """An infinity is not read twice where K ends in half a step of 128 columns."""
+    m, wq = _module(2, 128, in_f)
+    x = torch.randn(2 * rows, in_f, generator=torch.Generator().manual_seed(4)).bfloat16()
+    x[0, in_f - 1] = float("inf")
+    x[1, 0] = float("-inf")
+    x[rows + 1, in_f - 64] = float("nan")
+    y = _np(m.grouped_linear("w1", x.cuda(), offsets=torch.tensor([rows, 2 * rows], device="cuda")))
+    with np.errstate(invalid="ignore"):
+        want, _ = _reference(x.double().numpy(), wq.astype(np.float64), [rows, 2 * rows])
+    assert np.array_equal(np.isnan(y), np.isnan(want))
+    assert np.array_equal(np.isposinf(y), np.isposinf(want)) and np.array_equal(np.isneginf(y), np.isneginf(want))
+    assert np.isposinf(y[0]).any() and np.isnan(y[rows + 1]).all() and np.isfinite(y[2:rows + 1]).all()
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_bad_weights_spoil_their_column_only(bad):
     g = torch.Generator().manual_seed(0)
@@ -552,9 +569,10 @@ def test_chunks_and_expert_choice_train_over_mxfp4():
             _grad_close(a, c)
 
 
-@pytest.mark.parametrize("tokens,rank", [(1, 0), (9, 16), (200, 16), (700, 40)])
-def test_routed_layer_and_its_gradients(tokens, rank):
-    w = wl.Workload("mxfp4", 14, tokens, 256, 192, 8, 2, max(rank, 8), 16.0, "mxfp4", torch.bfloat16)
+@pytest.mark.parametrize("tokens,rank,hidden", [(1, 0, 256), (9, 16, 256), (200, 16, 256), (700, 40, 256),
+                                                (1, 16, 320), (90, 0, 320), (700, 16, 320)])
+def test_routed_layer_and_its_gradients(tokens, rank, hidden):
+    w = wl.Workload("mxfp4", 14, tokens, hidden, 192, 8, 2, max(rank, 8), 16.0, "mxfp4", torch.bfloat16)
     dense, lora = wl.dense_weights(w), wl.lora_factors(w) if rank else None
     m = build_module(w, dense, lora)
     ow = {k: torch.from_numpy(omx.roundtrip(t.float().numpy())).bfloat16() for k, t in dense.items()}
