@@ -81,17 +81,17 @@ __device__ __forceinline__ int tensor_of(const Args &a, int chunk) {
 }
 
 template <bool BF16>
-__device__ __forceinline__ void load(const void *p, int64_t i, int n, bool vec, float (&x)[kVec]) {
-  if (vec && n >= kVec) {
+__device__ __forceinline__ void load(const void *p, int64_t i, int n, float (&x)[kVec]) {
+  if (n >= kVec) {
     if constexpr (BF16) {
-      const u32x4 q = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + i);
+      const u32x4 q = *reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(p) + i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[2 * j] = __uint_as_float(q[j] << 16);
         x[2 * j + 1] = __uint_as_float(q[j] & 0xffff0000u);
       }
     } else {
-      const f32x4 *q = reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i);
+      const f32x4_any *q = reinterpret_cast<const f32x4_any *>(static_cast<const float *>(p) + i);
       const f32x4 lo = q[0], hi = q[1];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -111,14 +111,14 @@ __device__ __forceinline__ void load(const void *p, int64_t i, int n, bool vec, 
 }
 
 template <bool BF16>
-__device__ __forceinline__ void store(void *p, int64_t i, int n, bool vec, const float (&x)[kVec]) {
-  if (vec && n >= kVec) {
+__device__ __forceinline__ void store(void *p, int64_t i, int n, const float (&x)[kVec]) {
+  if (n >= kVec) {
     if constexpr (BF16) {
-      *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p) + i) =
+      *reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(p) + i) =
           u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
                 pack_bf16x2(x[6], x[7])};
     } else {
-      f32x4 *q = reinterpret_cast<f32x4 *>(static_cast<float *>(p) + i);
+      f32x4_any *q = reinterpret_cast<f32x4_any *>(static_cast<float *>(p) + i);
       q[0] = f32x4{x[0], x[1], x[2], x[3]};
       q[1] = f32x4{x[4], x[5], x[6], x[7]};
     }
@@ -229,7 +229,6 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Args a) {
   const int ti = tensor_of(a, blockIdx.x);
   const Tensor t = a.t[ti];
   const Scalars s = a.device ? a.device[t.index] : a.s;
-  const bool vec = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g)) & 15) == 0;
   const int64_t i0 = static_cast<int64_t>(static_cast<int>(blockIdx.x) - t.first_chunk) * kChunk +
                      kVec * static_cast<int64_t>(threadIdx.x);
   // The runs' places: whole blocks are taken, their elements past n as zeros.
@@ -240,8 +239,8 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Args a) {
     const int64_t i = i0 + u * (kThreads * kVec);
     if (i >= padded) break;
     const int n = static_cast<int>(max(min(t.n - i, int64_t(kVec)), int64_t(0)));
-    load<BF16>(t.p, i, n, vec, p[u]);
-    load<BF16>(t.g, i, n, vec, g[u]);
+    load<BF16>(t.p, i, n, p[u]);
+    load<BF16>(t.g, i, n, g[u]);
     const int64_t at = t.at + i;
     if constexpr (STATE8) {
       unpack<4, true>(*reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.m) + at),
@@ -249,8 +248,8 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Args a) {
       unpack<5, false>(*reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(a.v) + at),
                        a.ve[at / kBlock], v[u]);
     } else {
-      load<false>(a.m, at, kVec, true, m[u]);
-      load<false>(a.v, at, kVec, true, v[u]);
+      load<false>(a.m, at, kVec, m[u]);
+      load<false>(a.v, at, kVec, v[u]);
     }
   }
 #pragma unroll
@@ -261,7 +260,7 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Args a) {
     const int64_t at = t.at + i;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) update(a, s, g[u][j], p[u][j], m[u][j], v[u][j]);
-    store<BF16>(t.p, i, n, vec, p[u]);
+    store<BF16>(t.p, i, n, p[u]);
     if constexpr (STATE8) {
       // Padding stays zero.
 #pragma unroll
@@ -284,8 +283,8 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Args a) {
         a.ve[at / kBlock] = static_cast<uint8_t>(ve);
       }
     } else {
-      store<false>(a.m, at, kVec, true, m[u]);
-      store<false>(a.v, at, kVec, true, v[u]);
+      store<false>(a.m, at, kVec, m[u]);
+      store<false>(a.v, at, kVec, v[u]);
     }
   }
 }
@@ -319,7 +318,7 @@ __global__ __launch_bounds__(256) void moments_kernel(const uint8_t *codes, cons
   if (r >= runs) return;
   float x[kVec];
   unpack<EB, SIGNED>(reinterpret_cast<const uint2 *>(codes)[r], exponents[r / (kBlock / kVec)], x);
-  store<false>(out, kVec * r, kVec, true, x);
+  store<false>(out, kVec * r, kVec, x);
 }
 
 bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }

@@ -38,18 +38,18 @@ __device__ __forceinline__ uint32_t quantize8(const float (&v)[8], uint32_t &sca
   return c;
 }
 
-// Eight elements from p on as fp32 (16-byte aligned).
+// Eight elements from p on as fp32.
 template <bool BF16>
 __device__ __forceinline__ void load8(const void *p, int64_t at, float (&v)[8]) {
   if constexpr (BF16) {
-    const u32x4 q = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + at);
+    const u32x4 q = *reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(p) + at);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[2 * i] = __uint_as_float(q[i] << 16);
       v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
     }
   } else {
-    const f32x4 *q = reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + at);
+    const f32x4_any *q = reinterpret_cast<const f32x4_any *>(static_cast<const float *>(p) + at);
     const f32x4 a = q[0], b = q[1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -59,7 +59,7 @@ __device__ __forceinline__ void load8(const void *p, int64_t at, float (&v)[8]) 
   }
 }
 
-// The first n <= 8 of eight elements at any alignment, the others zero.
+// The first n <= 8 of eight elements, the others zero.
 template <bool BF16>
 __device__ __forceinline__ void load8_guarded(const void *p, int64_t at, int n, float (&v)[8]) {
 #pragma unroll

@@ -18,11 +18,10 @@ constexpr int kUnroll = 4;  // groups of 8 elements per thread
 // x 2048 in bf16 93 us, 5.0 TB/s read and written, where a copy reaches 5.1.
 template <bool BF16>
 __global__ __launch_bounds__(256) void quantize_kernel(const void *x, int64_t rows, int64_t cols,
-                                                       int64_t ldx, bool vec, uint8_t *codes,
-                                                       uint8_t *scales) {
+                                                       int64_t ldx, uint8_t *codes, uint8_t *scales) {
   const int64_t per_row = 4 * ((cols + kBlock - 1) / kBlock);
   const int64_t total = rows * per_row;
-  const bool flat = vec && ldx == cols && cols % kBlock == 0;
+  const bool flat = ldx == cols && cols % kBlock == 0;
   auto row_of = [&](int64_t g) -> int64_t {
     return total <= 0xffffffffll ? static_cast<uint32_t>(g) / static_cast<uint32_t>(per_row)
                                  : g / per_row;
@@ -38,7 +37,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void *x, int64_t ro
       continue;
     }
     const int64_t row = row_of(g), col = 8 * (g - row * per_row);
-    if (vec && col + 8 <= cols)
+    if (col + 8 <= cols)
       load8<BF16>(x, row * ldx + col, v[u]);
     else
       load8_guarded<BF16>(x, row * ldx + col, static_cast<int>(max(min(cols - col, int64_t(8)), int64_t(0))), v[u]);
@@ -58,11 +57,10 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void *x, int64_t ro
 // from the cache that the quantisation before it filled).
 template <bool BF16>
 __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t *codes, const uint8_t *scales,
-                                                         int64_t rows, int64_t cols, bool vec,
-                                                         void *out) {
+                                                         int64_t rows, int64_t cols, void *out) {
   const int64_t per_row = 4 * ((cols + kBlock - 1) / kBlock);
   const int64_t total = rows * per_row;
-  const bool flat = vec && cols % kBlock == 0;
+  const bool flat = cols % kBlock == 0;
   const int64_t g0 = static_cast<int64_t>(blockIdx.x) * (256 * kUnroll) + threadIdx.x;
   uint32_t c[kUnroll], e[kUnroll];
 #pragma unroll
@@ -96,8 +94,8 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t *codes, c
       u32x4 q;
 #pragma unroll
       for (int i = 0; i < 4; ++i) q[i] = pack_bf16x2(f[i][0], f[i][1]);
-      if (vec && left >= 8) {
-        *reinterpret_cast<u32x4 *>(o) = q;
+      if (left >= 8) {
+        *reinterpret_cast<u32x4_any *>(o) = q;
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -105,9 +103,9 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const uint8_t *codes, c
       }
     } else {
       float *o = static_cast<float *>(out) + at;
-      if (vec && left >= 8) {
-        reinterpret_cast<f32x4 *>(o)[0] = f32x4{f[0][0], f[0][1], f[1][0], f[1][1]};
-        reinterpret_cast<f32x4 *>(o)[1] = f32x4{f[2][0], f[2][1], f[3][0], f[3][1]};
+      if (left >= 8) {
+        reinterpret_cast<f32x4_any *>(o)[0] = f32x4{f[0][0], f[0][1], f[1][0], f[1][1]};
+        reinterpret_cast<f32x4_any *>(o)[1] = f32x4{f[2][0], f[2][1], f[3][0], f[3][1]};
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -245,8 +243,8 @@ __device__ void plan_tiles(const PlanOut &P) {
 // read and written; in order of the rows, with codes and scales of a row scattered over
 // the tiles, 155.
 template <bool BF16>
-__global__ __launch_bounds__(256) void rows_kernel(const void *x, int64_t rows, int64_t cols, bool vec,
-                                                   uint8_t *codes, uint8_t *scales, PlanOut P) {
+__global__ __launch_bounds__(256) void rows_kernel(const void *x, int64_t rows, int64_t cols, uint8_t *codes,
+                                                   uint8_t *scales, PlanOut P) {
   if (blockIdx.x == gridDim.x - 1) {
     plan_tiles(P);
     return;
@@ -262,11 +260,12 @@ __global__ __launch_bounds__(256) void rows_kernel(const void *x, int64_t rows, 
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int64_t row = row0 + 4 * u;
-    const int n = row < rows && col < cols ? 8 : 0;
-    if (vec && n)
+    if (row < rows && col < cols) {
       load8<BF16>(x, row * cols + col, v[u]);
-    else
-      load8_guarded<BF16>(x, row * cols + col, n, v[u]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+    }
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
@@ -536,10 +535,9 @@ extern "C" int mx_mxfp4_quantize(const void *x, int x_dtype, int64_t rows, int64
   const int64_t blocks = ceil_div(rows * 4 * ceil_div(cols, kBlock), 256 * kUnroll);
   if (int rc = grid_ok(name, blocks)) return rc;
   const bool bf16 = x_dtype == MX_DTYPE_BF16;
-  const bool vec = aligned16(x) && (ldx * (bf16 ? 2 : 4)) % 16 == 0;
   auto kernel = bf16 ? quantize_kernel<true> : quantize_kernel<false>;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, as_stream(stream), x,
-                     rows, cols, ldx, vec, codes, scales);
+                     rows, cols, ldx, codes, scales);
   return check_launch(name);
 }
 
@@ -559,10 +557,9 @@ extern "C" int mx_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, 
   const int64_t blocks = ceil_div(rows * 4 * ceil_div(cols, kBlock), 256 * kUnroll);
   if (int rc = grid_ok(name, blocks)) return rc;
   const bool bf16 = out_dtype == MX_DTYPE_BF16;
-  const bool vec = aligned16(out) && (cols * (bf16 ? 2 : 4)) % 16 == 0;
   auto kernel = bf16 ? dequantize_kernel<true> : dequantize_kernel<false>;
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, as_stream(stream),
-                     codes, scales, rows, cols, vec, out);
+                     codes, scales, rows, cols, out);
   return check_launch(name);
 }
 
@@ -620,7 +617,7 @@ extern "C" int mx_mxfp4_grouped_linear(const void *x, int x_dtype, const void *o
   const bool bf16 = x_dtype == MX_DTYPE_BF16;
   auto rows_k = bf16 ? rows_kernel<true> : rows_kernel<false>;
   hipLaunchKernelGGL(rows_k, dim3(static_cast<unsigned>(chunks + 1)), dim3(256), 0, s, x, num_rows, K,
-                     aligned16(x), codes, scales, P);
+                     codes, scales, P);
   if (int rc = check_launch(name)) return rc;
   Product p = {codes, scales, static_cast<const uint8_t *>(w->data),
                static_cast<const uint8_t *>(w->scale), num_rows, K, N, P.head, P.tall, P.rest,
